@@ -41,7 +41,7 @@ extern "C" {
 
 typedef struct CUstream_st* ufp8_stream_t; /* same handle as cudaStream_t */
 
-#define UFP8_ABI_VERSION 5
+#define UFP8_ABI_VERSION 6
 
 /* return codes */
 #define UFP8_OK 0
@@ -285,6 +285,60 @@ int ufp8_xent_combine(const float* stats, int64_t ld_stats, const void* logits_b
 int ufp8_xent_backward(const void* logits_bf16, int64_t rows, int64_t V, int64_t ldl, const int32_t* labels,
                        const uint8_t* mask, const float* lse, const float* qrow, const float* dloss, float cap,
                        int fmt, void* dlogits, int64_t ldo, float* amax, float* inv_scale, ufp8_stream_t stream);
+
+/* ---- token log probabilities and distillation on logit rows ------------------------------------
+ * Operators next to the cross-entropy above, on the same rows of logits; they have no counterpart
+ * in the reference, whose only use of the logits is that loss.  Row r of the logits is
+ * ptr + (r / inner) * stride_outer + (r % inner) * stride_inner elements, V columns of unit stride (so
+ * a next-token shift or a padded pitch needs no copy; any alignment of the rows is taken).  The
+ * distribution of a row is softmax(x / temperature).  mask: uint8 [rows] or NULL; a row whose mask is
+ * 0 is not read.  stats: f32 [rows][4], 16-byte aligned, kept for the backward (NULL: not wanted). */
+typedef struct ufp8_logit_rows {
+  const void* ptr;
+  int32_t dtype;     /* UFP8_OUT_BF16 / UFP8_OUT_F32 */
+  float temperature; /* > 0 */
+  int64_t rows, V;
+  int64_t inner; /* >= 1 */
+  int64_t stride_outer, stride_inner;
+  const uint8_t* mask;
+} ufp8_logit_rows;
+
+/* Per row: logprob = log softmax[token], entropy = -sum p log p, and the top_k (0..256, <= V) largest
+ * logits in descending order as (log probability, column), NaN first and ties to the lowest column.
+ * tokens: int32 or int64 (token_bytes 4 / 8), a negative one counts from the end, one outside
+ * [-V, V) gives NaN.  Any of the outputs may be NULL (tokens and logprob together).  A masked row
+ * gives 0, 0, (-inf, -1).  A column of -inf has probability 0; a row of only -inf, or with +inf or
+ * NaN, gives NaN.  One launch. */
+int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens, int token_bytes, int64_t top_k,
+                         float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, float* stats,
+                         ufp8_stream_t stream);
+/* dlogits (the logits' type; row r at (r / inner) * out_stride_outer + (r % inner) * out_stride_inner
+ * elements, rows apart) for the upstream gradients dlogprob and dentropy (f32, one per row at the given
+ * stride; 0: one value for all rows) and dtop (f32 [rows][top_k], with the forward's top_ids); NULL:
+ * none.  dentropy needs a forward with `entropy`.  A masked row's gradient is 0.  Every column of every
+ * row is written; fastest where an output row starts as far from a 16-byte boundary as its logit row. */
+int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const void* tokens, int token_bytes,
+                          const float* dlogprob, int64_t dlogprob_stride, const float* dentropy,
+                          int64_t dentropy_stride, const float* dtop, const int64_t* top_ids, int64_t top_k,
+                          void* dlogits, int64_t out_stride_outer, int64_t out_stride_inner,
+                          ufp8_stream_t stream);
+
+/* Distillation from a teacher's top logits.  Per row, `entries` (0..1024) columns teacher_ids (int32 or
+ * int64) with the teacher's logits or log probabilities there (UFP8_OUT_BF16 / UFP8_OUT_F32), both
+ * [rows][entries]; an id < 0 marks an absent entry.  q = softmax(teacher / temperature) over the
+ * entries present, p = softmax(x / temperature) over all V columns:
+ *   loss = sum_j q_j (log q_j - log p[id_j]),
+ * the Kullback-Leibler divergence from the teacher's distribution renormalised over its entries.
+ * Entries of -inf have q = 0; a row without any weight, or masked, has loss 0; an id >= V with q > 0
+ * gives NaN.  A column given twice counts twice. */
+int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teacher_ids, int id_bytes, const void* teacher,
+                         int teacher_dtype, int64_t entries, float* loss, float* stats, ufp8_stream_t stream);
+/* dlogits[v] = dloss / temperature * (p_v - sum of q_j with id_j == v), 0 for rows with loss 0 by the
+ * rules above; arguments as in ufp8_logprob_backward.  The teacher gets no gradient. */
+int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stats, const void* teacher_ids, int id_bytes,
+                          const void* teacher, int teacher_dtype, int64_t entries, const float* dloss,
+                          int64_t dloss_stride, void* dlogits, int64_t out_stride_outer,
+                          int64_t out_stride_inner, ufp8_stream_t stream);
 
 /* ---- Newton-Schulz orthogonalisation (Muon) ------------------------------------------------
  * Replaces orthogonalize (ueaj/opt/multiscale.py:110-141): optax.contrib's

@@ -57,6 +57,10 @@ EXPORTED_SYMBOLS = (
     "ufp8_xent_forward",
     "ufp8_xent_combine",
     "ufp8_xent_backward",
+    "ufp8_logprob_forward",
+    "ufp8_logprob_backward",
+    "ufp8_distill_forward",
+    "ufp8_distill_backward",
     "ufp8_newton_schulz_workspace",
     "ufp8_newton_schulz",
     "ufp8_rope_table",
@@ -126,6 +130,20 @@ class GemmDesc(ctypes.Structure):
         ("attn_row", ctypes.c_void_p),
         ("attn_scale", ctypes.c_float),
         ("attn_reserved", ctypes.c_int32),
+    ]
+
+
+class LogitRows(ctypes.Structure):
+    _fields_ = [
+        ("ptr", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("rows", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("inner", ctypes.c_int64),
+        ("stride_outer", ctypes.c_int64),
+        ("stride_inner", ctypes.c_int64),
+        ("mask", ctypes.c_void_p),
     ]
 
 
@@ -199,6 +217,11 @@ def load() -> ctypes.CDLL:
     lib.ufp8_xent_forward.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, vp, vp]
     lib.ufp8_xent_combine.argtypes = [vp, i64, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp]
     lib.ufp8_xent_backward.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, vp, f32, i32, vp, i64, vp, vp, vp]
+    rp = ctypes.POINTER(LogitRows)
+    lib.ufp8_logprob_forward.argtypes = [rp, vp, i32, i64, vp, vp, vp, vp, vp, vp]
+    lib.ufp8_logprob_backward.argtypes = [rp, vp, vp, i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, i64, vp]
+    lib.ufp8_distill_forward.argtypes = [rp, vp, i32, vp, i32, i64, vp, vp, vp]
+    lib.ufp8_distill_backward.argtypes = [rp, vp, vp, i32, vp, i32, i64, vp, i64, vp, i64, i64, vp]
     lib.ufp8_newton_schulz_workspace.argtypes = [i64, i64, i64, ctypes.POINTER(i64)]
     lib.ufp8_newton_schulz.argtypes = [vp, i32, i64, i64, i64, i32, vp, f32, vp, i32, vp, i64, vp]
     lib.ufp8_rope_table.argtypes = [vp, i64, i64, vp, vp, vp, vp]
@@ -214,6 +237,7 @@ def load() -> ctypes.CDLL:
                  "ufp8_tp_local", "ufp8_tp_ag_push", "ufp8_tp_set_copy_lanes", "ufp8_tp_rs_push_copy",
                  "ufp8_rmsnorm_quant", "ufp8_rmsnorm_backward_workspace",
                  "ufp8_rmsnorm_backward", "ufp8_xent_forward", "ufp8_xent_combine", "ufp8_xent_backward",
+                 "ufp8_logprob_forward", "ufp8_logprob_backward", "ufp8_distill_forward", "ufp8_distill_backward",
                  "ufp8_newton_schulz_workspace", "ufp8_newton_schulz", "ufp8_rope_table", "ufp8_rope",
                  "ufp8_attention_workspace", "ufp8_attention_forward", "ufp8_attention_backward"):
         getattr(lib, name).restype = i32
@@ -299,6 +323,37 @@ def xent_backward(logits_ptr, rows, V, ldl, labels_ptr, mask_ptr, lse_ptr, qrow_
     check(load().ufp8_xent_backward(logits_ptr, rows, V, ldl, labels_ptr, mask_ptr, lse_ptr, qrow_ptr, dloss_ptr,
                                     cap, fmt, out_ptr, ldo, amax_ptr, inv_ptr, stream))
     _count((1 if fmt != BF16 else 0) + (1 if rows > 0 else 0))
+
+
+def logprob_forward(rows: LogitRows, tokens_ptr, token_bytes, top_k, logprob_ptr, entropy_ptr, top_lp_ptr, top_id_ptr,
+                    stats_ptr, stream) -> None:
+    """ufp8_logprob_forward: log probabilities of given tokens, entropy and top alternatives."""
+    check(load().ufp8_logprob_forward(ctypes.byref(rows), tokens_ptr, token_bytes, top_k, logprob_ptr, entropy_ptr,
+                                      top_lp_ptr, top_id_ptr, stats_ptr, stream))
+    _count(1 if rows.rows > 0 else 0)
+
+
+def logprob_backward(rows: LogitRows, stats_ptr, tokens_ptr, token_bytes, dlp_ptr, dlp_stride, dent_ptr, dent_stride,
+                     dtop_ptr, top_id_ptr, top_k, out_ptr, out_outer, out_inner, stream) -> None:
+    check(load().ufp8_logprob_backward(ctypes.byref(rows), stats_ptr, tokens_ptr, token_bytes, dlp_ptr, dlp_stride,
+                                       dent_ptr, dent_stride, dtop_ptr, top_id_ptr, top_k, out_ptr, out_outer,
+                                       out_inner, stream))
+    _count(1 if rows.rows > 0 else 0)
+
+
+def distill_forward(rows: LogitRows, ids_ptr, id_bytes, teacher_ptr, teacher_dtype, entries, loss_ptr, stats_ptr,
+                    stream) -> None:
+    """ufp8_distill_forward: the loss against a teacher's top logits."""
+    check(load().ufp8_distill_forward(ctypes.byref(rows), ids_ptr, id_bytes, teacher_ptr, teacher_dtype, entries,
+                                      loss_ptr, stats_ptr, stream))
+    _count(1 if rows.rows > 0 else 0)
+
+
+def distill_backward(rows: LogitRows, stats_ptr, ids_ptr, id_bytes, teacher_ptr, teacher_dtype, entries, dloss_ptr,
+                     dloss_stride, out_ptr, out_outer, out_inner, stream) -> None:
+    check(load().ufp8_distill_backward(ctypes.byref(rows), stats_ptr, ids_ptr, id_bytes, teacher_ptr, teacher_dtype,
+                                       entries, dloss_ptr, dloss_stride, out_ptr, out_outer, out_inner, stream))
+    _count(1 if rows.rows > 0 else 0)
 
 
 def newton_schulz_workspace(batch: int, m: int, n: int) -> int:

@@ -518,6 +518,143 @@ def head_xent_backward(dloss: torch.Tensor, saved, labels: torch.Tensor, mask: t
     return dxn, dw
 
 
+# ----------------------------------------------------------------------------- logit rows
+# Operators on rows of logits [..., V] next to the loss: log probabilities of given tokens with
+# entropy and top alternatives, and distillation from a teacher's top logits (csrc/logprob.cu).
+_LOGIT_DTYPE = {torch.bfloat16: C.OUT_BF16, torch.float32: C.OUT_F32}
+
+
+@dataclass(frozen=True)
+class LogitRows:
+    """The rows of a logits tensor [..., V] as the kernels address them (include/ufp8.h).  `logits` is
+    the tensor itself, or a contiguous copy where its strides have more than two levels."""
+    logits: torch.Tensor
+    rows: int
+    inner: int
+    stride_outer: int
+    stride_inner: int
+
+    def c(self, temperature: float, mask: torch.Tensor | None) -> C.LogitRows:
+        t = self.logits
+        return C.LogitRows(t.data_ptr(), _LOGIT_DTYPE[t.dtype], temperature, self.rows, t.shape[-1], self.inner,
+                           self.stride_outer, self.stride_inner, mask.data_ptr() if mask is not None else None)
+
+
+def logit_rows(logits: torch.Tensor) -> LogitRows:
+    V = logits.shape[-1]
+    if logits.is_contiguous():
+        rows = logits.numel() // V
+        return LogitRows(logits, rows, max(rows, 1), 0, V)
+    if logits.numel() == 0 or (V > 1 and logits.stride(-1) != 1):
+        return logit_rows(logits.contiguous())
+    levels = []  # (size, stride) of the leading dimensions, outermost first, merged where they are one walk
+    for size, stride in zip(logits.shape[:-1], logits.stride()[:-1]):
+        if size == 1:
+            continue
+        if levels and levels[-1][1] == stride * size:
+            levels[-1] = (levels[-1][0] * size, stride)
+        else:
+            levels.append((size, stride))
+    if len(levels) > 2:
+        return logit_rows(logits.contiguous())
+    inner, stride_inner = levels[-1] if levels else (1, V)
+    outer, stride_outer = levels[0] if len(levels) == 2 else (1, 0)
+    return LogitRows(logits, outer * inner, inner, stride_outer, stride_inner)
+
+
+def _grad_rows(lr: LogitRows):
+    """(gradient tensor of the logits' shape, row strides): contiguous for contiguous logits on a
+    16-byte boundary; otherwise each row starts as far from such a boundary as its logit row (the
+    backward then loads and stores 16 bytes at a time), by a few elements between the rows."""
+    t = lr.logits
+    V, e = t.shape[-1], 16 // t.element_size()
+    start = (t.data_ptr() // t.element_size()) % e
+    inner = V + (lr.stride_inner - V) % e
+    outer = lr.inner * inner + (lr.stride_outer - lr.inner * inner) % e if lr.rows > lr.inner else lr.inner * inner
+    if start == 0 and t.is_contiguous():
+        return torch.empty_like(t), 0, V
+    n_outer = lr.rows // lr.inner
+    buf = torch.empty(start + n_outer * outer, dtype=t.dtype, device=t.device)
+    return buf.as_strided((n_outer, lr.inner, V), (outer, inner, 1), start).view(t.shape), outer, inner
+
+
+def token_logprobs_forward(lr: LogitRows, tokens: torch.Tensor | None, mask: torch.Tensor | None, top_k: int,
+                           temperature: float, entropy: bool, want_stats: bool):
+    """(logprob, entropy, top log probabilities, top ids, stats) over the flattened rows; None where not
+    asked for (ufp8_logprob_forward)."""
+    t, rows = lr.logits, lr.rows
+    dev, V = t.device, t.shape[-1]
+    f32 = {"dtype": torch.float32, "device": dev}
+    lp = torch.empty(rows, **f32) if tokens is not None else None
+    ent = torch.empty(rows, **f32) if entropy else None
+    top_lp = torch.empty((rows, top_k), **f32) if top_k else None
+    top_id = torch.empty((rows, top_k), dtype=torch.int64, device=dev) if top_k else None
+    stats = torch.empty((rows, 4), **f32) if want_stats else None
+    ptr = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
+    with torch.cuda.device(dev):
+        _launch("logprob", float(t.element_size()) * rows * V, lambda: C.logprob_forward(
+            lr.c(temperature, mask), ptr(tokens), tokens.element_size() if tokens is not None else 0, top_k, ptr(lp),
+            ptr(ent), ptr(top_lp), ptr(top_id), ptr(stats), _stream()))
+    return lp, ent, top_lp, top_id, stats
+
+
+def _row_grad(g: torch.Tensor | None):
+    """An upstream gradient of one f32 per row as (tensor, elements between rows): 0 for one value
+    expanded over the rows (what .sum() and .mean() send back)."""
+    if g is None:
+        return None, 0
+    g = g.to(torch.float32)
+    if not any(g.stride()):
+        return g, 0
+    return g.contiguous(), 1
+
+
+def token_logprobs_backward(lr: LogitRows, stats: torch.Tensor, tokens: torch.Tensor | None, mask: torch.Tensor | None,
+                            temperature: float, dlp: torch.Tensor | None, dent: torch.Tensor | None,
+                            dtop: torch.Tensor | None, top_id: torch.Tensor | None) -> torch.Tensor:
+    """dlogits of token_logprobs_forward (ufp8_logprob_backward)."""
+    t, rows = lr.logits, lr.rows
+    dlp, s_lp = _row_grad(dlp)
+    dent, s_ent = _row_grad(dent)
+    dtop = None if dtop is None else dtop.to(torch.float32).contiguous()
+    top_k = top_id.shape[-1] if dtop is not None else 0
+    ptr = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
+    with torch.cuda.device(t.device):
+        out, outer, inner = _grad_rows(lr)
+        _launch("logprob_grad", 2.0 * t.element_size() * rows * t.shape[-1], lambda: C.logprob_backward(
+            lr.c(temperature, mask), stats.data_ptr(), ptr(tokens), tokens.element_size() if tokens is not None else 0,
+            ptr(dlp), s_lp, ptr(dent), s_ent, ptr(dtop), ptr(top_id), top_k, out.data_ptr(), outer, inner, _stream()))
+    return out
+
+
+def distill_forward(lr: LogitRows, ids: torch.Tensor, teacher: torch.Tensor, mask: torch.Tensor | None,
+                    temperature: float, want_stats: bool):
+    """(loss, stats) over the flattened rows (ufp8_distill_forward)."""
+    t, rows = lr.logits, lr.rows
+    loss = torch.empty(rows, dtype=torch.float32, device=t.device)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=t.device) if want_stats else None
+    with torch.cuda.device(t.device):
+        _launch("distill", float(t.element_size()) * rows * t.shape[-1], lambda: C.distill_forward(
+            lr.c(temperature, mask), ids.data_ptr(), ids.element_size(), teacher.data_ptr(),
+            _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], loss.data_ptr(),
+            stats.data_ptr() if stats is not None else None, _stream()))
+    return loss, stats
+
+
+def distill_backward(lr: LogitRows, stats: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
+                     mask: torch.Tensor | None, temperature: float, dloss: torch.Tensor) -> torch.Tensor:
+    """dlogits of distill_forward (ufp8_distill_backward)."""
+    t, rows = lr.logits, lr.rows
+    dloss, stride = _row_grad(dloss)
+    with torch.cuda.device(t.device):
+        out, outer, inner = _grad_rows(lr)
+        _launch("distill_grad", 2.0 * t.element_size() * rows * t.shape[-1], lambda: C.distill_backward(
+            lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(), ids.element_size(), teacher.data_ptr(),
+            _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride, out.data_ptr(), outer, inner,
+            _stream()))
+    return out
+
+
 # ----------------------------------------------------------------------------- Newton-Schulz
 def newton_schulz(g: torch.Tensor, coeffs, eps: float = 1e-8, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """ufp8_newton_schulz over g [batch, m, n] (f32 or bf16, CUDA): the orthogonalisation of Muon
