@@ -13,8 +13,7 @@
 //   rowstat_kernel   one CTA per row streams the row once, a running (m, s, t) per thread,
 //                    and in the same pass keeps the candidates for the top alternatives.
 //   rowgrad_kernel   the gradient of both operators: p_v (A + B log2 p_v) with row factors A, B, plus
-//                    weights at a few columns (the token, the alternatives, the teacher's entries),
-//                    which overwrite the dense value after it was stored.
+//                    weights at a few columns (the token, the alternatives, the teacher's entries).
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -109,11 +108,12 @@ struct Row {
     p = static_cast<const typename T::raw*>(base) + elem;
     off = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(typename T::raw));
     V = v;
-    units = static_cast<int>((static_cast<int64_t>(v) + off + 7) >> 3);
+    units = (v + off + 7) >> 3;
   }
-  __device__ __forceinline__ int64_t col(int i) const { return static_cast<int64_t>(i) * 8 - off; }
+  // V < 2^31 - 2^20: a column a tile past the row's end still fits
+  __device__ __forceinline__ int col(int i) const { return i * 8 - off; }
   __device__ __forceinline__ Unit<T> load(int i) const {
-    const int64_t c = col(i);
+    const int c = col(i);
     Unit<T> u;
     if (c >= 0 && c + 8 <= V) {
 #pragma unroll
@@ -145,13 +145,19 @@ struct RowsArgs {
   float inv_t;  // 1 / temperature
 };
 
-__device__ __forceinline__ int64_t row_elem(int64_t r, int64_t inner, int64_t stride_outer, int64_t stride_inner) {
-  const int64_t o = r / inner;
-  return o * stride_outer + (r - o * inner) * stride_inner;
-}
-__device__ __forceinline__ int64_t row_elem(const RowsArgs& a, int64_t r) {
-  return row_elem(r, a.inner, a.stride_outer, a.stride_inner);
-}
+// Row r as (outer, inner) indices: 32-bit arithmetic, since rows < 2^31, and none for one level.
+struct RowIndex {
+  int o, i;
+  __device__ __forceinline__ RowIndex(const RowsArgs& a, int r) : o(0), i(r) {
+    if (a.rows > a.inner) {
+      o = static_cast<unsigned>(r) / static_cast<unsigned>(a.inner);
+      i = r - o * static_cast<int>(a.inner);
+    }
+  }
+  __device__ __forceinline__ int64_t elem(int64_t stride_outer, int64_t stride_inner) const {
+    return o * stride_outer + i * stride_inner;
+  }
+};
 
 __device__ __forceinline__ int64_t load_id(const void* p, int bytes, int64_t i) {
   return bytes == 8 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(kThreads) rowstat_kernel(const StatArgs a) {
   extern __shared__ uint64_t keys[];  // kTop: kCand
   __shared__ Stat sh_stat[kWarps];
   __shared__ TopShared sh;
-  const int64_t row = blockIdx.x;
+  const int row = blockIdx.x;
   const int tid = threadIdx.x;
   const float c2 = a.r.c2;
 
@@ -413,13 +419,13 @@ __global__ void __launch_bounds__(kThreads) rowstat_kernel(const StatArgs a) {
       if (a.stats) a.stats[row] = make_float4(kNegInf, 0.0f, kDistill ? kNegInf : 0.0f, 0.0f);
     }
     if (kTop && tid < a.k) {
-      a.top_lp[row * a.k + tid] = kNegInf;
-      a.top_id[row * a.k + tid] = -1;
+      a.top_lp[static_cast<int64_t>(row) * a.k + tid] = kNegInf;
+      a.top_id[static_cast<int64_t>(row) * a.k + tid] = -1;
     }
     return;
   }
 
-  const Row<T> x(a.r.x, row_elem(a.r, row), a.r.V);
+  const Row<T> x(a.r.x, RowIndex(a.r, row).elem(a.r.stride_outer, a.r.stride_inner), a.r.V);
   Stat st{kNegInf, 0.0f, 0.0f};
   float tau = kNegInf;     // every one of the k largest so far is >= tau ...
   bool inclusive = true;   // ... and a later element equal to it may still belong to them
@@ -468,7 +474,7 @@ __global__ void __launch_bounds__(kThreads) rowstat_kernel(const StatArgs a) {
         if (inclusive ? !(mx[u] < tau) : !(mx[u] <= tau)) {
           float v[8];
           unpack<T>(w[u], v);
-          const int64_t c = x.col(u0 + u * kThreads + tid);
+          const int c = x.col(u0 + u * kThreads + tid);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             if ((inclusive ? !(v[j] < tau) : !(v[j] <= tau)) && c + j >= 0 && c + j < x.V) {
@@ -545,8 +551,8 @@ __global__ void __launch_bounds__(kThreads) rowstat_kernel(const StatArgs a) {
         for (int i = 0; i < n; ++i) rank += keys[i] > key;
         const uint32_t col = key_col(key, a.ib);
         const float xv = T::to_f(x.p[col]);
-        a.top_lp[row * a.k + rank] = __fmaf_rn(__fsub_rn(xv, r.m), a.r.inv_t, -ls);
-        a.top_id[row * a.k + rank] = col;
+        a.top_lp[static_cast<int64_t>(row) * a.k + rank] = __fmaf_rn(__fsub_rn(xv, r.m), a.r.inv_t, -ls);
+        a.top_id[static_cast<int64_t>(row) * a.k + rank] = col;
       }
     }
   }
@@ -576,123 +582,205 @@ struct GradArgs {
   int64_t dloss_stride;
   void* out;
   int64_t out_outer, out_inner;  // row strides of the output
-  int chunks;  // work units of a row
+  int tasks;     // tasks of a row
+  int per_task;  // chunks of a task
 };
 
-struct EntryShared {
-  int id[kMaxEntries];
-  float w[kMaxEntries];
-  float total;
-};
+// Two f32 at once (one issue slot of the FMA pipe for both).
+__device__ __forceinline__ uint64_t pk(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpk(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 
+// Entry j < n of a row: its column (-1: none) and the value that its weight comes from.
+template <bool kDistill>
+__device__ __forceinline__ void load_entry(const GradArgs& a, int64_t row, int j, int* id, float* val) {
+  if constexpr (kDistill) {
+    const int64_t e = row * a.K + j;
+    const int64_t i = load_id(a.ids, a.id_bytes, e);
+    *id = (i >= 0 && i < a.r.V) ? static_cast<int>(i) : -1;
+    *val = a.teacher_f32 ? static_cast<const float*>(a.teacher)[e]
+                         : Bf16::to_f(static_cast<const uint16_t*>(a.teacher)[e]);
+  } else if (a.dlogprob && j == 0) {
+    *id = token_col(load_id(a.tokens, a.token_bytes, row), a.r.V);
+    *val = a.dlogprob[row * a.dlogprob_stride];
+  } else {
+    const int64_t e = row * a.k + j - (a.dlogprob ? 1 : 0);
+    *id = static_cast<int>(a.top_id[e]);
+    *val = a.dtop[e];
+  }
+}
+
+// The warps of a resident grid walk (row, task) units on their own, without a barrier; a task is `per_task`
+// chunks of a row, a chunk 2 KB of it, kUnits 16-byte loads a lane.  Per task the warp works out the row
+// factors; per chunk it adds the weights of the row's entries that fall into it into `wt`, one f32 per
+// column and zero elsewhere, in entry order, so that the result does not depend on timing.  Then
+// v = p * factor + weight, and a lane with a weight in its columns sets those back to zero.
 template <class T, bool kDistill>
-__global__ void __launch_bounds__(kThreads) rowgrad_kernel(const GradArgs a) {
-  __shared__ EntryShared sh;
-  constexpr int kChunk = kThreads * T::kUnits;  // units of a chunk
-  const int tid = threadIdx.x;
-  const float c2 = a.r.c2;
-  const int64_t work = a.r.rows * a.chunks;
-  for (int64_t wi = blockIdx.x; wi < work; wi += gridDim.x) {
-    const int64_t row = wi / a.chunks;
-    const int u0 = static_cast<int>(wi - row * a.chunks) * kChunk;
-    const Row<T> x(a.r.x, row_elem(a.r, row), a.r.V);
-    typename T::raw* o = static_cast<typename T::raw*>(a.out) + row_elem(row, a.r.inner, a.out_outer, a.out_inner);
+__global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) {
+  constexpr int kChunk = 32 * T::kUnits;  // units of a chunk
+  extern __shared__ float4 wt_all[];      // kWarps * kChunk * 8 floats
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float4* wt4 = wt_all + warp * kChunk * 2;
+  float* wt = reinterpret_cast<float*>(wt4);
+  // unit wi = (row, task) = (wi / tasks, wi % tasks), advanced by the grid's warps without divisions
+  const int rows = static_cast<int>(a.r.rows);
+  const unsigned first = blockIdx.x * kWarps + warp, step = gridDim.x * kWarps;
+  const int step_r = static_cast<int>(step / a.tasks), step_t = static_cast<int>(step % a.tasks);
+  int row = static_cast<int>(first / a.tasks), task = static_cast<int>(first % a.tasks);
+  const uint64_t c22 = pk(a.r.c2, a.r.c2);
+  const int n = kDistill ? a.K : (a.dlogprob ? 1 : 0) + (a.dtop ? a.k : 0);
+  if (n > 0)
+    for (int i = lane; i < kChunk * 2; i += 32) wt4[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __syncwarp();
+  for (; row < rows; row += step_r, task += step_t) {
+    if (task >= a.tasks) {
+      task -= a.tasks;
+      if (++row >= rows) break;
+    }
+    const RowIndex ri(a.r, row);
+    const Row<T> x(a.r.x, ri.elem(a.r.stride_outer, a.r.stride_inner), a.r.V);
+    typename T::raw* o = static_cast<typename T::raw*>(a.out) + ri.elem(a.out_outer, a.out_inner);
     const bool vec = ((reinterpret_cast<uintptr_t>(o) ^ reinterpret_cast<uintptr_t>(x.p)) & 15u) == 0;
     const float4 st = a.stats[row];
     const bool dead = (a.r.mask && a.r.mask[row] == 0) || (kDistill && st.z == kNegInf);
+    int u0 = task * a.per_task * kChunk;
+    const int u_end = min(u0 + a.per_task * kChunk, x.units);
     float A = 0.0f, B = 0.0f;
-    int n = 0;
-    __syncthreads();  // the previous unit's entries are no longer read
+    int id0 = -1;  // the first 32 entries stay with their lanes
+    float val0 = 0.0f;
     if (!dead) {
+      if (lane < n) load_entry<kDistill>(a, row, lane, &id0, &val0);
       if constexpr (kDistill) {
         A = __fmul_rn(a.dloss[row * a.dloss_stride], a.r.inv_t);
-        n = a.K;
-        for (int j = tid; j < n; j += kThreads) {
-          const int64_t id = load_id(a.ids, a.id_bytes, row * a.K + j);
-          const int64_t e = row * a.K + j;
-          const float tv = a.teacher_f32 ? static_cast<const float*>(a.teacher)[e]
-                                         : Bf16::to_f(static_cast<const uint16_t*>(a.teacher)[e]);
-          sh.id[j] = (id >= 0 && id < a.r.V) ? static_cast<int>(id) : -1;
-          sh.w[j] = __fmul_rn(-A, ex2a(__fmaf_rn(__fsub_rn(tv, st.z), c2, -st.w)));
-        }
       } else {
-        float g = a.dlogprob ? __fmul_rn(a.dlogprob[row * a.dlogprob_stride], a.r.inv_t) : 0.0f;
+        const float g = a.dlogprob ? __fmul_rn(a.dlogprob[row * a.dlogprob_stride], a.r.inv_t) : 0.0f;
         const float h = a.dentropy ? __fmul_rn(a.dentropy[row * a.dentropy_stride], a.r.inv_t) : 0.0f;
-        n = (a.dlogprob ? 1 : 0) + (a.dtop ? a.k : 0);
-        if (tid == 0 && a.dlogprob) {
-          sh.id[0] = token_col(load_id(a.tokens, a.token_bytes, row), a.r.V);
-          sh.w[0] = g;
-        }
+        float top = 0.0f;
         if (a.dtop) {
-          const int first = a.dlogprob ? 1 : 0;
-          for (int j = tid; j < a.k; j += kThreads) {
-            sh.id[first + j] = static_cast<int>(a.top_id[row * a.k + j]);
-            sh.w[first + j] = __fmul_rn(a.dtop[row * a.k + j], a.r.inv_t);
-          }
-          __syncthreads();
-          if (tid == 0) {
-            float sum = 0.0f;
-            for (int j = 0; j < a.k; ++j) sum = __fadd_rn(sum, sh.w[first + j]);
-            sh.total = sum;
-          }
-          __syncthreads();
-          g = __fadd_rn(g, sh.total);
+          for (int j = lane; j < a.k; j += 32)
+            top = __fmaf_rn(a.dtop[static_cast<int64_t>(row) * a.k + j], a.r.inv_t, top);
+          top = warp_sum(top);
         }
-        A = -__fmaf_rn(h, st.z, g);
+        A = -__fmaf_rn(h, st.z, __fadd_rn(g, top));
         B = __fmul_rn(-h, kLn2);
       }
     }
-    auto dense = [&](float v) {
-      // log2 p; the clamp as in fold8
-      const float u = maxn(__fmaf_rn(__fsub_rn(v, st.x), c2, -st.y), -160.0f);
-      return __fmul_rn(ex2a(u), kDistill ? A : __fmaf_rn(B, u, A));
-    };
+    const uint64_t nm = pk(-st.x, -st.x), nl = pk(-st.y, -st.y);
+    const uint64_t A2 = pk(A, A), B2 = pk(B, B);
+    for (; u0 < u_end; u0 += kChunk) {
+      const int lo = x.col(u0), hi = x.col(u0 + kChunk);
+      const bool whole = lo >= 0 && hi <= x.V && vec;  // every unit is 16-byte loads and stores
+      Unit<T> w[T::kUnits];
+      unsigned flag = 0;  // bit u: unit u of this lane holds a weight
+      if (!dead) {
+        if (whole) {
+          const uint4* p = reinterpret_cast<const uint4*>(x.p + lo) + lane * T::kWords;
 #pragma unroll
-    for (int u = 0; u < T::kUnits; ++u) {
-      const int i = u0 + u * kThreads + tid;
-      if (i >= x.units) continue;
-      float v[8];
-      if (dead) {
+          for (int u = 0; u < T::kUnits; ++u)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-      } else {
-        unpack<T>(x.load(i), v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = dense(v[j]);
-      }
-      const int64_t c = x.col(i);
-      if (vec && c >= 0 && c + 8 <= x.V) {
-        if constexpr (T::kWords == 1) {
-          uint4 q;
-          uint32_t* qw = &q.x;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            qw[j] = *reinterpret_cast<const uint32_t*>(&b);
-          }
-          *reinterpret_cast<uint4*>(o + c) = q;
+            for (int k = 0; k < T::kWords; ++k) w[u].w[k] = ld16(p + u * 32 * T::kWords + k);
         } else {
-          reinterpret_cast<float4*>(o + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
-          reinterpret_cast<float4*>(o + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+          for (int u = 0; u < T::kUnits; ++u) {
+            const int i = u0 + u * 32 + lane;
+            if (i < x.units) w[u] = x.load(i);
+          }
         }
-      } else {
-        for (int j = 0; j < 8; ++j)
-          if (c + j >= 0 && c + j < x.V) o[c + j] = T::from_f(v[j]);
+        for (int j0 = 0; j0 < n; j0 += 32) {
+          int id = id0;
+          float val = val0;
+          if (j0 > 0) {
+            id = -1;
+            if (j0 + lane < n) load_entry<kDistill>(a, row, j0 + lane, &id, &val);
+          }
+          const bool in = id >= 0 && id >= lo && id < hi;
+          const unsigned active = __ballot_sync(0xFFFFFFFFu, in);
+          if (active == 0) continue;
+          const float ew = kDistill ? __fmul_rn(-A, ex2a(__fmaf_rn(__fsub_rn(val, st.z), a.r.c2, -st.w)))
+                                    : __fmul_rn(val, a.r.inv_t);
+          const int at = id - lo;
+          for (unsigned left = active; left; left &= left - 1) {  // in entry order
+            const int src = __ffs(left) - 1;
+            const int sat = __shfl_sync(0xFFFFFFFFu, at, src);
+            const float sw = __shfl_sync(0xFFFFFFFFu, ew, src);
+            if (lane == ((sat >> 3) & 31)) {  // the lane that owns the column
+              wt[sat] = __fadd_rn(wt[sat], sw);
+              flag |= 1u << (sat >> 8);
+            }
+          }
+        }
       }
-    }
-    if (dead || n == 0) continue;
-    __syncthreads();  // the entries are complete, and the dense values are stored before these overwrite them
-    const int64_t lo = x.col(u0), hi = x.col(u0 + kChunk);
-    for (int j = tid; j < n; j += kThreads) {
-      const int id = sh.id[j];
-      if (id < 0 || id < lo || id >= hi) continue;
-      bool first = true;  // a column given more than once is written once, by its first entry
-      for (int i = 0; i < j; ++i) first = first && sh.id[i] != id;
-      if (!first) continue;
-      float w = 0.0f;
-      for (int i = j; i < n; ++i)
-        if (sh.id[i] == id) w = __fadd_rn(w, sh.w[i]);
-      o[id] = T::from_f(__fadd_rn(dense(T::to_f(x.p[id])), w));
+#pragma unroll
+      for (int u = 0; u < T::kUnits; ++u) {
+        const int i = u0 + u * 32 + lane;
+        if (!whole && i >= x.units) continue;
+        float v[8];
+        if (dead) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        } else {
+          unpack<T>(w[u], v);
+          float e[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+          if ((flag >> u) & 1u) {
+            float4* q = wt4 + (u * 32 + lane) * 2;
+            const float4 q0 = q[0], q1 = q[1];
+            e[0] = q0.x, e[1] = q0.y, e[2] = q0.z, e[3] = q0.w, e[4] = q1.x, e[5] = q1.y, e[6] = q1.z, e[7] = q1.w;
+            q[0] = q[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            // log2 p; below -160 the power is 0 and 0 * log2 p has to stay 0
+            float z0, z1;
+            unpk(fma2(add2(pk(v[j], v[j + 1]), nm), c22, nl), z0, z1);
+            if (!kDistill) {
+              z0 = maxn(z0, -160.0f);
+              z1 = maxn(z1, -160.0f);
+            }
+            const uint64_t f = kDistill ? A2 : fma2(B2, pk(z0, z1), A2);
+            unpk(fma2(pk(ex2a(z0), ex2a(z1)), f, pk(e[j], e[j + 1])), v[j], v[j + 1]);
+          }
+        }
+        const int c = x.col(i);
+        if (whole || (vec && c >= 0 && c + 8 <= x.V)) {
+          if constexpr (T::kWords == 1) {
+            uint4 q;
+            uint32_t* qw = &q.x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+              qw[j] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            *reinterpret_cast<uint4*>(o + c) = q;
+          } else {
+            reinterpret_cast<float4*>(o + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(o + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (c + j >= 0 && c + j < x.V) o[c + j] = T::from_f(v[j]);
+        }
+      }
     }
   }
 }
@@ -759,12 +847,28 @@ int launch_logprob(const StatArgs& a, bool ent, cudaStream_t s) {
 
 template <class T, bool kDistill>
 int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
-  constexpr int kChunk = kThreads * T::kUnits;
+  constexpr int kChunk = 32 * T::kUnits;
   // a row that starts off a 16-byte boundary can need one unit more
-  a.chunks = static_cast<int>(((static_cast<int64_t>(a.r.V) + 7) / 8 + 1 + kChunk - 1) / kChunk);
-  const int64_t work = a.r.rows * a.chunks;
-  const int64_t cap = static_cast<int64_t>(dev.sm_count) * 8;
-  rowgrad_kernel<T, kDistill><<<static_cast<unsigned>(work < cap ? work : cap), kThreads, 0, s>>>(a);
+  const int64_t chunks = ((static_cast<int64_t>(a.r.V) + 7) / 8 + 1 + kChunk - 1) / kChunk;
+  const bool entries = kDistill ? a.K > 0 : (a.dlogprob || a.dtop);
+  const size_t smem = entries ? sizeof(float) * 8 * kChunk * kWarps : 0;
+  // one wave: CTAs beyond the resident ones would start when the first are done
+  static thread_local int dev_of[2] = {-1, -1}, per_sm[2] = {0, 0};
+  if (dev_of[entries] != dev.device) {
+    int n = 0;
+    const cudaError_t e =
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rowgrad_kernel<T, kDistill>, kThreads, smem);
+    if (e != cudaSuccess) return cuda_error(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor(row gradient)");
+    per_sm[entries] = n < 1 ? 1 : n;
+    dev_of[entries] = dev.device;
+  }
+  const int64_t cap = static_cast<int64_t>(dev.sm_count) * per_sm[entries];
+  // Longer tasks spread the row's set-up over more columns, as long as every warp still gets several.
+  a.per_task = 1;
+  while (a.per_task < 4 && a.per_task < chunks && a.r.rows * chunks >= cap * kWarps * 8 * a.per_task) a.per_task *= 2;
+  a.tasks = static_cast<int>((chunks + a.per_task - 1) / a.per_task);
+  const int64_t work = (a.r.rows * a.tasks + kWarps - 1) / kWarps;
+  rowgrad_kernel<T, kDistill><<<static_cast<unsigned>(work < cap ? work : cap), kThreads, smem, s>>>(a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? UFP8_OK : cuda_error(e, "row gradient launch");
 }
