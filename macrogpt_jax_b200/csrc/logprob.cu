@@ -14,6 +14,7 @@
 //                    and in the same pass keeps the candidates for the top alternatives.
 //   rowgrad_kernel   the gradient of both operators: p_v (A + B log2 p_v) with row factors A, B, plus
 //                    weights at a few columns (the token, the alternatives, the teacher's entries).
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -23,10 +24,8 @@
 namespace ufp8 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of a gradient CTA; a statistics CTA has 256 or 64
 constexpr int kWarps = kThreads / 32;
-constexpr int kSub = kThreads * 8;  // columns that one unit (8 elements) of every thread covers
-constexpr int kCand = 4096;         // candidate keys of a CTA; >= kMaxTop + kSub
 constexpr int kMaxTop = 256;
 constexpr int kMaxEntries = 1024;   // teacher entries of a row
 constexpr float kLn2 = 0.6931471805599453f;
@@ -169,64 +168,114 @@ __device__ __forceinline__ int token_col(int64_t t, int V) {
   return (t >= 0 && t < V) ? static_cast<int>(t) : -1;
 }
 
+// Two f32 at once (one issue slot of the FMA pipe for both).
+__device__ __forceinline__ uint64_t pk(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpk(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // ---- running softmax statistics -----------------------------------------------------------------
 struct Stat {
   float m, s, t;
 };
 
-// (m, s, t) <- (m, s, t) + (m2, s2, t2).  A NaN in either part makes s NaN.
-__device__ __forceinline__ void merge(Stat& a, const Stat& b, float c2) {
-  const float M = maxn(a.m, b.m);
-  if (M == kNegInf) return;  // both empty
-  // 2^-1000 is 0, and the clamp keeps 0 * d finite
-  const float da = a.m == kNegInf ? -1000.0f : maxn(__fmul_rn(a.m - M, c2), -1000.0f);
-  const float db = b.m == kNegInf ? -1000.0f : maxn(__fmul_rn(b.m - M, c2), -1000.0f);
-  const float fa = ex2a(da), fb = ex2a(db);
-  a.t = __fadd_rn(__fmul_rn(fa, __fmaf_rn(da, a.s, a.t)), __fmul_rn(fb, __fmaf_rn(db, b.s, b.t)));
-  a.s = __fadd_rn(__fmul_rn(fa, a.s), __fmul_rn(fb, b.s));
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_maxn(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = maxn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+
+// (s, t) moved to the maximum M >= a.m.  -1000: the power is 0, and 0 times the clamped d stays 0
+// (an empty part, m = -inf, has s = t = 0).
+__device__ __forceinline__ void rescale(Stat& a, float M, float c2) {
+  const float d = a.m == kNegInf ? -1000.0f : maxn(__fmul_rn(__fsub_rn(a.m, M), c2), -1000.0f);
+  const float f = ex2a(d);
+  a.t = __fmul_rn(f, __fmaf_rn(d, a.s, a.t));
+  a.s = __fmul_rn(f, a.s);
   a.m = M;
 }
 
-// Eight values into the running statistics; cm is their maximum (NaN if one is NaN).
-template <bool kEnt>
-__device__ __forceinline__ void fold8(const float (&v)[8], float cm, Stat& a, float c2) {
-  if (!(cm <= a.m)) {
-    const float d = a.m == kNegInf ? -1000.0f : maxn(__fmul_rn(a.m - cm, c2), -1000.0f);
-    const float f = ex2a(d);
-    if (kEnt) a.t = __fmul_rn(f, __fmaf_rn(d, a.s, a.t));
-    a.s = __fmul_rn(f, a.s);
-    a.m = cm;
-  }
-  const float mz = a.m == kNegInf ? 0.0f : a.m;
-  float s = 0.0f, t = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    // -160: below the smallest f32, so the power is 0, and 0 * z stays 0 for z = -inf
-    const float z = maxn(__fmul_rn(__fsub_rn(v[j], mz), c2), -160.0f);
-    const float e = ex2a(z);
-    s = __fadd_rn(s, e);
-    if (kEnt) t = __fmaf_rn(e, z, t);
-  }
-  a.s = __fadd_rn(a.s, s);
-  if (kEnt) a.t = __fadd_rn(a.t, t);
+// The merge of the lanes' parts, the same in every lane.  A NaN makes s NaN.
+__device__ __forceinline__ Stat warp_merge(Stat a, float c2) {
+  rescale(a, warp_maxn(a.m), c2);
+  a.s = warp_sum(a.s);
+  a.t = warp_sum(a.t);
+  return a;
 }
 
-// The CTA's statistics, merged lane by lane (a butterfly that is commutative bit for bit) and then
-// warp by warp; valid in thread 0 .. 31 after the barrier inside.
-__device__ __forceinline__ Stat block_merge(Stat a, Stat* sh, float c2) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat b;
-    b.m = __shfl_xor_sync(0xFFFFFFFFu, a.m, o);
-    b.s = __shfl_xor_sync(0xFFFFFFFFu, a.s, o);
-    b.t = __shfl_xor_sync(0xFFFFFFFFu, a.t, o);
-    merge(a, b, c2);
+// The maximum of a unit, NaN if one of its elements is.
+template <class T>
+__device__ __forceinline__ float unit_max(const Unit<T>& u) {
+  if constexpr (T::kWords == 1) {
+    uint32_t a, b;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(u.w[0].x), "r"(u.w[0].y));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(u.w[0].z), "r"(u.w[0].w));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+    return maxn(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
+  } else {
+    float v[8];
+    unpack<T>(u, v);
+    return maxn(maxn(maxn(v[0], v[1]), maxn(v[2], v[3])), maxn(maxn(v[4], v[5]), maxn(v[6], v[7])));
   }
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
-  __syncthreads();
-  Stat r = sh[0];
-  for (int w = 1; w < kWarps; ++w) merge(r, sh[w], c2);
-  return r;
+}
+
+// A thread's units of one tile into its running statistics; cm is their maximum.
+template <class T, bool kEnt>
+__device__ __forceinline__ void fold_tile(const Unit<T> (&w)[T::kUnits], float cm, Stat& a, float c2) {
+  if (!(cm <= a.m)) rescale(a, cm, c2);
+  const float mz = a.m == kNegInf ? 0.0f : a.m;
+  const uint64_t nm = pk(-mz, -mz), c22 = pk(c2, c2);
+  uint64_t s = 0, t = 0;
+#pragma unroll
+  for (int u = 0; u < T::kUnits; ++u) {
+    float v[8];
+    unpack<T>(w[u], v);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      float z0, z1;
+      uint64_t z = mul2(add2(pk(v[j], v[j + 1]), nm), c22);
+      unpk(z, z0, z1);
+      if (kEnt) {  // below the smallest f32 the power is 0, and 0 * z has to stay 0 for z = -inf
+        z0 = maxn(z0, -160.0f);
+        z1 = maxn(z1, -160.0f);
+        z = pk(z0, z1);
+      }
+      const uint64_t e = pk(ex2a(z0), ex2a(z1));
+      s = add2(s, e);
+      if (kEnt) t = fma2(e, z, t);
+    }
+  }
+  float lo, hi;
+  unpk(s, lo, hi);
+  a.s = __fadd_rn(a.s, __fadd_rn(lo, hi));
+  if (kEnt) {
+    unpk(t, lo, hi);
+    a.t = __fadd_rn(a.t, __fadd_rn(lo, hi));
+  }
 }
 
 // ---- the largest k of a row ---------------------------------------------------------------------
@@ -251,50 +300,132 @@ __device__ __forceinline__ uint32_t key_col(uint64_t key, int ib) {
   return static_cast<uint32_t>(((1ull << ib) - 1ull) - (key & ((1ull << ib) - 1ull)));
 }
 
-struct TopShared {
-  uint32_t hist[256];
-  int cnt;
-  int bin, above, in_bin;
-  float tau[kWarps];
-};
-
-// keys[0, n) -> those >= bound (and, with below_col >= 0, of a column < below_col), in any order at
-// keys[0, sh.cnt).  Whole CTA; ends with a barrier.
-__device__ __forceinline__ int filter_keys(uint64_t* keys, int n, uint64_t bound, int64_t below_col, int ib,
-                                           TopShared& sh) {
-  __syncthreads();
-  if (threadIdx.x == 0) sh.cnt = 0;
-  for (int b = 0; b < n; b += kThreads) {
-    const int i = b + static_cast<int>(threadIdx.x);
-    const uint64_t key = i < n ? keys[i] : 0;
-    const bool keep = i < n && key >= bound && (below_col < 0 || key_col(key, ib) < below_col);
-    __syncthreads();  // this block is read before anything is written to it
-    if (keep) keys[atomicAdd(&sh.cnt, 1)] = key;
-  }
-  __syncthreads();
-  const int left = sh.cnt;
-  __syncthreads();
-  return left;
+// The float of a 32-bit order (the value bits of an F32 key).
+__device__ __forceinline__ float order_value(uint32_t o) {
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
+// The upper 16 bits of x's order.
+template <class T>
+__device__ __forceinline__ uint32_t order16(float x) {
+  return static_cast<uint32_t>(make_key<T>(x, 0, 1) >> (T::kKeyBits - 16 + 1));
 }
 
-// Keeps the k largest of keys[0, n), n > k, by radix selection from the key's top bits in digits of
-// eight; returns a bound b with exactly k keys >= b.  Whole CTA.
-__device__ uint64_t keep_largest(uint64_t* keys, int n, int k, int bits, int ib, TopShared& sh) {
+constexpr int kRegion = 512;  // candidate keys of a warp; at least kMaxTop + the 256 columns of a unit
+constexpr int kSlots = 32;    // entries per thread of the table of maxima
+constexpr int kFinal = 256;   // keys that are put in order by comparing all with all; >= kMaxTop
+constexpr int kMaxParts = 8;  // CTAs of a cluster that share a row
+
+// Shared memory for the search, by CTA size: the table (kSlots x kThr orders), the items and the gathered keys, or,
+// once those are of no use, a region per warp.
+template <int kThr>
+struct TopLayout {
+  static constexpr int kItems = 4 * kThr;
+  static constexpr int kGather = kThr == 256 ? 1024 : 512;
+  static constexpr size_t kTableBytes = sizeof(uint16_t) * kSlots * kThr;
+  static constexpr size_t kItemBytes = sizeof(uint32_t) * kItems;
+  static constexpr size_t kFast = kTableBytes + kItemBytes + sizeof(uint64_t) * kGather;
+  static constexpr size_t kSlow = sizeof(uint64_t) * kRegion * (kThr / 32);
+  static constexpr size_t kBytes = kFast > kSlow ? kFast : kSlow;
+};
+
+template <int kThr>
+struct TopShared {
+  uint32_t hist[256];
+  uint32_t maxima[kThr];  // order16 of a thread's maximum over the even / odd slots of the table
+  uint32_t reached;       // order16 that at least k elements of the CTA's columns reach (0: not known)
+  int items, n;
+  int bin, above, in_bin;
+  uint64_t last[kFinal];
+  float m, ls;
+};
+
+// What the CTAs of a cluster bring to the first one of it.
+struct PartsShared {
+  Stat stat[kMaxParts];
+  int count[kMaxParts];
+};
+
+// The largest 16-bit order that at least k of the maxima reach, found bit by bit by one warp; 0 where there
+// are fewer than k.  Each maximum stands for an element of its own, so k elements reach the result.
+template <int kThr>
+__device__ __forceinline__ uint32_t reached_by(const uint32_t* maxima, int k) {
+  constexpr int kPer = kThr / 32;
+  const bool halves = k > kThr / 2;  // two values per thread: closer for a large k
+  uint32_t lo[kPer], hi[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t w = maxima[i * 32 + (threadIdx.x & 31)];
+    lo[i] = w & 0xFFFFu;
+    hi[i] = w >> 16;
+    if (!halves) lo[i] = max(lo[i], hi[i]);
+  }
+  uint32_t b = 0;
+#pragma unroll 1
+  for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+    const uint32_t c = b | bit;
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) cnt += lo[i] >= c;
+    if (halves) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) cnt += hi[i] >= c;
+    }
+    if (__reduce_add_sync(0xFFFFFFFFu, cnt) >= k) b = c;
+  }
+  return b;
+}
+// The float just below all of an order16's: two steps, since one step below 0 is the order of -0, which
+// compares as 0.  NaN, which nothing is <= to, for 0 and for the order of -inf.
+__device__ __forceinline__ float below_order(uint32_t reached) {
+  return reached ? order_value((reached << 16) - 2u) : __int_as_float(0x7FC00000);
+}
+
+// One warp: leaves the k largest of keys[0, n), n > k, in keys[0, k); returns a bound b with exactly k
+// keys >= b.
+__device__ __noinline__ uint64_t warp_keep_largest(uint64_t* keys, int n, int k, int bits) {
+  const int lane = threadIdx.x & 31;
+  uint64_t b = 0;
+  for (int bit = bits - 1; bit >= 0; --bit) {
+    const uint64_t c = b | (1ull << bit);
+    int cnt = 0;
+    for (int i = lane; i < n; i += 32) cnt += keys[i] >= c;
+    cnt = __reduce_add_sync(0xFFFFFFFFu, cnt);
+    if (cnt >= k) b = c;
+    if (cnt == k) break;
+  }
+  int left = 0;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const uint64_t key = i0 + lane < n ? keys[i0 + lane] : 0;
+    const bool keep = i0 + lane < n && key >= b;
+    const unsigned who = __ballot_sync(0xFFFFFFFFu, keep);  // all of these are read before one is written
+    if (keep) keys[left + __popc(who & ((1u << lane) - 1u))] = key;
+    left += __popc(who);
+    __syncwarp();
+  }
+  return b;
+}
+
+// A bound b with exactly k keys >= b among the warps' lists, which hold more than k: radix selection from
+// the key's top bits in digits of eight.  Whole CTA; begins and ends with a barrier.
+template <int kThr>
+__device__ uint64_t select_bound(const uint64_t* mine, int n_mine, int k, int bits, TopShared<kThr>& sh) {
+  const int lane = threadIdx.x & 31;
   uint64_t bound = 0;
   int need = k, shift = bits;
+  __syncthreads();
   while (shift > 0) {
     const int w = shift < 8 ? shift : 8;
     const int top = shift;
     shift -= w;
-    sh.hist[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < 256; i += kThr) sh.hist[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint64_t key = keys[i];
+    for (int i = lane; i < n_mine; i += 32) {
+      const uint64_t key = mine[i];
       if ((key >> top) == (bound >> top)) atomicAdd(&sh.hist[(key >> shift) & ((1u << w) - 1u)], 1u);
     }
     __syncthreads();
     if (threadIdx.x < 32) {  // lane l holds bins 255 - 8 l ... 248 - 8 l, largest first
-      const int hi = 255 - 8 * static_cast<int>(threadIdx.x);
+      const int hi = 255 - 8 * lane;
       int sum = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += static_cast<int>(sh.hist[hi - j]);
@@ -302,7 +433,7 @@ __device__ uint64_t keep_largest(uint64_t* keys, int n, int k, int bits, int ib,
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xFFFFFFFFu, pre, o);
-        if (static_cast<int>(threadIdx.x) >= o) pre += up;
+        if (lane >= o) pre += up;
       }
       int before = pre - sum;
       if (before < need && pre >= need) {  // exactly one lane
@@ -321,21 +452,72 @@ __device__ uint64_t keep_largest(uint64_t* keys, int n, int k, int bits, int ib,
     __syncthreads();
     bound |= static_cast<uint64_t>(sh.bin) << shift;
     need -= sh.above;
-    if (sh.in_bin == need) break;  // the whole bin belongs to the k largest
-    __syncthreads();               // everyone has read the choice before the next digit
+    const bool whole = sh.in_bin == need;  // the whole bin belongs to the k largest
+    __syncthreads();                       // everyone has read the choice before the next digit
+    if (whole) break;
   }
-  filter_keys(keys, n, bound, -1, ib, sh);
   return bound;
 }
+
+// A warp's search of a whole row for candidates, for rows with more elements at the bound than fit.  An
+// element is a candidate if it is above `thr`, below which k elements of the row lie: either those that
+// `reached` vouches for (equal elements included, since those k may stand further right), or k of the
+// warp's own earlier columns (equal elements excluded).  A NaN threshold lets everything through.
+template <class T>
+struct Search {
+  uint64_t* keys;  // kRegion
+  int n = 0;
+  int k, ib;
+  float thr;
+  __device__ __forceinline__ Search(uint64_t* region, int k_, int ib_, uint32_t reached)
+      : keys(region), k(k_), ib(ib_), thr(below_order(reached)) {}
+  // unit: 8 columns from c on for every lane, right of all columns before
+  __device__ __forceinline__ void take(const Unit<T>& unit, float mx, int c, int V) {
+    unsigned hit = 0;
+    if (!(mx <= thr)) {
+      float v[8];
+      unpack<T>(unit, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) hit |= !(v[j] <= thr) ? 1u << j : 0u;
+      if (c < 0) hit &= 0xFFu << min(-c, 8);
+      if (c + 8 > V) hit &= 0xFFu >> min(c + 8 - V, 8);
+    }
+    unsigned who = __ballot_sync(0xFFFFFFFFu, hit != 0);
+    if (who == 0) return;
+    if (n > kRegion - 256) {
+      const float own = key_value<T>(warp_keep_largest(keys, n, k, T::kKeyBits + ib), ib);
+      n = k;
+      thr = fmaxf(thr, own);  // the one that is not NaN
+    }
+    const int lane = threadIdx.x & 31;
+    do {
+      if (hit) {
+        const int j = __ffs(hit) - 1;
+        hit &= hit - 1;
+        float v[8];
+        unpack<T>(unit, v);
+        float x = v[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) x = i == j ? v[i] : x;
+        keys[n + __popc(who & ((1u << lane) - 1u))] = make_key<T>(x, static_cast<uint32_t>(c + j), ib);
+      }
+      n += __popc(who);
+      who = __ballot_sync(0xFFFFFFFFu, hit != 0);
+    } while (who);
+    __syncwarp();
+  }
+};
 
 // ---- forward ------------------------------------------------------------------------------------
 struct StatArgs {
   RowsArgs r;
+  int part_bits;  // log2 of the CTAs that share a row
   // token_logprobs
   const void* tokens;  // may be null
   int token_bytes;
   int k;
-  int ib;  // column bits of a key
+  int ib;   // column bits of a key
+  int cap;  // keys that a CTA brings to the first one of its cluster
   float* logprob;
   float* entropy;
   float* top_lp;
@@ -354,204 +536,351 @@ struct StatArgs {
 __device__ __forceinline__ float teacher_val(const StatArgs& a, int64_t i) {
   return a.teacher_f32 ? static_cast<const float*>(a.teacher)[i] : Bf16::to_f(static_cast<const uint16_t*>(a.teacher)[i]);
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-  return v;
-}
-__device__ __forceinline__ float warp_maxn(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = maxn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-  return v;
+// A teacher entry: its column's logit (NaN: an id past the last column) and the teacher's value there.
+struct Entry {
+  bool has;
+  float t, x;
+};
+template <class T>
+__device__ __forceinline__ Entry teacher_entry(const StatArgs& a, int64_t e, const Row<T>& x) {
+  const int64_t id = load_id(a.ids, a.id_bytes, e);
+  Entry r{id >= 0, kNegInf, __int_as_float(0x7FC00000)};
+  if (r.has) r.t = teacher_val(a, e);
+  if (r.has && id < a.r.V) r.x = T::to_f(x.p[id]);
+  return r;
 }
 
 // One warp: the row's loss sum_j q_j (log q_j - log p_{id_j}) over the entries with id >= 0, and the
 // teacher's (max, log2 sum).  Entries whose teacher value is -inf have q = 0 and contribute 0; a row
-// without any weight has loss 0 (and max -inf, which the gradient reads as "no entry").
+// without any weight has loss 0 (and max -inf, which the gradient reads as "no entry").  The first 64
+// entries come loaded.
 template <class T>
-__device__ __forceinline__ float distill_row(const StatArgs& a, int64_t row, const Row<T>& x, float m, float ls,
-                                             float* tm_out, float* tl_out) {
+__device__ __forceinline__ float distill_row(const StatArgs& a, int64_t base, const Row<T>& x, const Entry (&first)[2],
+                                             float m, float ls, float* tm_out, float* tl_out) {
   const int lane = threadIdx.x & 31;
   const float c2 = a.r.c2;
-  const int64_t base = row * a.K;
-  float tm = kNegInf;
-  for (int j = lane; j < a.K; j += 32)
+  float tm = maxn(first[0].t, first[1].t);
+  for (int j = 64 + lane; j < a.K; j += 32)
     if (load_id(a.ids, a.id_bytes, base + j) >= 0) tm = maxn(tm, teacher_val(a, base + j));
   tm = warp_maxn(tm);
   *tm_out = tm;
   *tl_out = 0.0f;
   if (tm == kNegInf) return 0.0f;
   float ts = 0.0f;
-  for (int j = lane; j < a.K; j += 32)
+  for (int k = 0; k < 2; ++k)
+    if (first[k].has) ts = __fadd_rn(ts, ex2a(__fmul_rn(__fsub_rn(first[k].t, tm), c2)));
+  for (int j = 64 + lane; j < a.K; j += 32)
     if (load_id(a.ids, a.id_bytes, base + j) >= 0)
       ts = __fadd_rn(ts, ex2a(__fmul_rn(__fsub_rn(teacher_val(a, base + j), tm), c2)));
   ts = warp_sum(ts);
   const float tl = log2f(ts), tls = logf(ts);
   *tl_out = tl;
   float sum = 0.0f;
-  for (int j = lane; j < a.K; j += 32) {
-    const int64_t id = load_id(a.ids, a.id_bytes, base + j);
-    if (id < 0) continue;
-    const float td = __fsub_rn(teacher_val(a, base + j), tm);
+  auto add = [&](const Entry& e) {
+    const float td = __fsub_rn(e.t, tm);
     const float q = ex2a(__fmaf_rn(td, c2, -tl));
-    if (q == 0.0f) continue;
-    const float xv = id < a.r.V ? T::to_f(x.p[id]) : __int_as_float(0x7FC00000);
-    const float lp = __fmaf_rn(__fsub_rn(xv, m), a.r.inv_t, -ls);
+    if (!e.has || q == 0.0f) return;
+    const float lp = __fmaf_rn(__fsub_rn(e.x, m), a.r.inv_t, -ls);
     sum = __fmaf_rn(q, __fsub_rn(__fmaf_rn(td, a.r.inv_t, -tls), lp), sum);
-  }
+  };
+  add(first[0]);
+  add(first[1]);
+  for (int j = 64 + lane; j < a.K; j += 32) add(teacher_entry(a, base + j, x));
   return warp_sum(sum);
 }
 
-template <class T, bool kEnt, bool kTop, bool kDistill>
-__global__ void __launch_bounds__(kThreads) rowstat_kernel(const StatArgs a) {
-  extern __shared__ uint64_t keys[];  // kTop: kCand
-  __shared__ Stat sh_stat[kWarps];
-  __shared__ TopShared sh;
-  const int row = blockIdx.x;
+// What a statistics kernel computes besides (m, s).
+enum Mode { kPlain = 0, kEntropy = 1, kTopK = 2, kTeacher = 3 };  // kTopK: with the entropy
+
+template <class T, int kThr>
+__device__ __forceinline__ void load_tile(const Row<T>& x, int u0, int u_end, Unit<T> (&w)[T::kUnits]) {
   const int tid = threadIdx.x;
+  constexpr int kTile = kThr * T::kUnits;
+  if (u0 + kTile <= u_end && x.col(u0) >= 0 && x.col(u0 + kTile) <= x.V) {
+    const uint4* p = reinterpret_cast<const uint4*>(x.p + x.col(u0)) + tid * T::kWords;
+#pragma unroll
+    for (int u = 0; u < T::kUnits; ++u)
+#pragma unroll
+      for (int k = 0; k < T::kWords; ++k) w[u].w[k] = ld16(p + u * kThr * T::kWords + k);
+  } else {
+    constexpr uint32_t kFill = T::kWords == 1 ? 0xFF80FF80u : 0xFF800000u;  // -inf
+#pragma unroll
+    for (int u = 0; u < T::kUnits; ++u) {
+      const int i = u0 + u * kThr + tid;
+      if (i < u_end)
+        w[u] = x.load(i);
+      else
+        w[u].w[0] = w[u].w[T::kWords - 1] = make_uint4(kFill, kFill, kFill, kFill);
+    }
+  }
+}
+
+// The k largest of the CTA's units [u_begin, u_end), and a few more, as keys: this warp's list (*mine, *n_mine);
+// returns the number of all warps.  `reached` is a bound that k of the elements reach.  Its table says which
+// thread and which tiles saw a maximum that reaches it; those (little more than k) are read once more.
+// Where too many elements equal the bound (a constant row, say), the row is searched as a whole.
+template <class T, int kThr>
+__device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end, int per_slot, int slots, int k, int ib,
+                                        char* mem, TopShared<kThr>& sh, const uint64_t** mine, int* n_mine) {
+  using L = TopLayout<kThr>;
+  constexpr int kTile = kThr * T::kUnits;
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const uint16_t* table = reinterpret_cast<const uint16_t*>(mem);
+  uint32_t* items = reinterpret_cast<uint32_t*>(mem + L::kTableBytes);
+  uint64_t* gather = reinterpret_cast<uint64_t*>(mem + L::kTableBytes + L::kItemBytes);
+  const uint32_t reached = sh.reached;
+  const float thr = below_order(reached);
+  for (int slot = 0; slot < slots; ++slot)
+    if (table[slot * kThr + tid] >= reached) {
+      const int at = atomicAdd(&sh.items, 1);
+      if (at < L::kItems) items[at] = static_cast<uint32_t>(slot << 16 | tid);
+    }
+  __syncthreads();
+  const int m = sh.items;
+  if (m <= L::kItems) {
+    for (int it = tid; it < m; it += kThr) {
+      const int slot = items[it] >> 16, t = items[it] & 0xFFFFu;
+      for (int tile = slot * per_slot; tile < (slot + 1) * per_slot; ++tile) {
+        Unit<T> w[T::kUnits];
+#pragma unroll
+        for (int u = 0; u < T::kUnits; ++u) {
+          const int i = u_begin + tile * kTile + u * kThr + t;
+          if (i < u_end) w[u] = x.load(i);
+        }
+#pragma unroll
+        for (int u = 0; u < T::kUnits; ++u) {
+          const int i = u_begin + tile * kTile + u * kThr + t;
+          if (i >= u_end || unit_max<T>(w[u]) <= thr) continue;
+          float v[8];
+          unpack<T>(w[u], v);
+          const int c = x.col(i);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!(v[j] <= thr) && c + j >= 0 && c + j < x.V) {
+              const int at = atomicAdd(&sh.n, 1);
+              if (at < L::kGather) gather[at] = make_key<T>(v[j], static_cast<uint32_t>(c + j), ib);
+            }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = sh.n;
+  if (m <= L::kItems && n <= L::kGather) {
+    const int per = (n + kThr / 32 - 1) / (kThr / 32);
+    *mine = gather + warp * per;
+    *n_mine = max(0, min(per, n - warp * per));
+    return n;
+  }
+  __syncthreads();  // the table, the items and the gathered keys give way to the regions
+  Search<T> top(reinterpret_cast<uint64_t*>(mem) + warp * kRegion, k, ib, reached);
+  if (tid == 0) sh.n = 0;
+  for (int u0 = u_begin; u0 < u_end; u0 += kTile) {
+    Unit<T> w[T::kUnits];
+    load_tile<T, kThr>(x, u0, u_end, w);
+#pragma unroll
+    for (int u = 0; u < T::kUnits; ++u)
+      top.take(w[u], unit_max<T>(w[u]), x.col(u0 + u * kThr + tid), x.V);
+  }
+  *mine = top.keys;
+  *n_mine = top.n;
+  __syncthreads();
+  if ((tid & 31) == 0) atomicAdd(&sh.n, top.n);
+  __syncthreads();
+  return sh.n;
+}
+
+// The warps' lists, cut to exactly k keys if they hold more than `most` (>= k, <= room of out), into out in any order;
+// returns their number.  Whole CTA; begins and ends with a barrier.
+template <int kThr>
+__device__ __forceinline__ int collect(const uint64_t* mine, int n_mine, int n, int k, int most, int bits,
+                                       uint64_t* out, TopShared<kThr>& sh) {
+  const uint64_t bound = n > most ? select_bound<kThr>(mine, n_mine, k, bits, sh) : 0;
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  for (int i = threadIdx.x & 31; i < n_mine; i += 32)
+    if (mine[i] >= bound) out[atomicAdd(&sh.n, 1)] = mine[i];
+  __syncthreads();
+  return n > most ? k : n;
+}
+
+// One CTA per row, or a cluster of 2 to 8 that share a row's units and bring their parts to the first of them.
+template <class T, int kThr, int kMode>
+__global__ void __launch_bounds__(kThr) rowstat_kernel(const StatArgs a) {
+  constexpr bool kEnt = kMode == kEntropy || kMode == kTopK;
+  constexpr bool kTop = kMode == kTopK;
+  constexpr int kNWarps = kThr / 32;
+  constexpr int kTile = kThr * T::kUnits;  // units of a tile
+  extern __shared__ __align__(16) char mem[];  // kTop: TopLayout, then the keys of the cluster's CTAs
+  __shared__ Stat sh_stat[kNWarps];
+  __shared__ PartsShared parts;
+  __shared__ TopShared<kTop ? kThr : 32> sh;
+  const int row = blockIdx.x >> a.part_bits, n_parts = 1 << a.part_bits;
+  const int part = blockIdx.x & (n_parts - 1);
+  const int tid = threadIdx.x, warp = tid >> 5;
   const float c2 = a.r.c2;
 
   if (a.r.mask && a.r.mask[row] == 0) {  // nothing of the row is read
+    if (part > 0) return;
     if (tid == 0) {
       if (a.logprob) a.logprob[row] = 0.0f;
       if (a.entropy) a.entropy[row] = 0.0f;
-      if (kDistill) a.loss[row] = 0.0f;
-      if (a.stats) a.stats[row] = make_float4(kNegInf, 0.0f, kDistill ? kNegInf : 0.0f, 0.0f);
+      if (kMode == kTeacher) a.loss[row] = 0.0f;
+      if (a.stats) a.stats[row] = make_float4(kNegInf, 0.0f, kMode == kTeacher ? kNegInf : 0.0f, 0.0f);
     }
-    if (kTop && tid < a.k) {
-      a.top_lp[static_cast<int64_t>(row) * a.k + tid] = kNegInf;
-      a.top_id[static_cast<int64_t>(row) * a.k + tid] = -1;
-    }
+    if constexpr (kTop)
+      for (int j = tid; j < a.k; j += kThr) {
+        a.top_lp[static_cast<int64_t>(row) * a.k + j] = kNegInf;
+        a.top_id[static_cast<int64_t>(row) * a.k + j] = -1;
+      }
     return;
   }
+  namespace cg = cooperative_groups;
+  if (n_parts > 1) cg::this_cluster().barrier_arrive();  // "started", awaited before the others' memory is used
 
   const Row<T> x(a.r.x, RowIndex(a.r, row).elem(a.r.stride_outer, a.r.stride_inner), a.r.V);
-  Stat st{kNegInf, 0.0f, 0.0f};
-  float tau = kNegInf;     // every one of the k largest so far is >= tau ...
-  bool inclusive = true;   // ... and a later element equal to it may still belong to them
-  if (kTop && tid == 0) sh.cnt = 0;
+  // This CTA's units; parts begin at a multiple of 8 units (128 bytes of bf16).
+  const int per_part = n_parts == 1 ? x.units : (((x.units + n_parts - 1) >> a.part_bits) + 7) & ~7;
+  const int u_begin = min(part * per_part, x.units), u_end = min(u_begin + per_part, x.units);
 
-  constexpr int kTile = kThreads * T::kUnits;  // units of a tile
-  for (int u0 = 0; u0 < x.units; u0 += kTile) {
+  // The few logits that the row's results need by column, before the stream.
+  float x_tok = __int_as_float(0x7FC00000);
+  Entry entry[2];
+  if constexpr (kMode == kTeacher) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      entry[k].has = false;
+      entry[k].t = kNegInf;
+      if (part == 0 && tid < 32 && k * 32 + tid < a.K)
+        entry[k] = teacher_entry(a, static_cast<int64_t>(row) * a.K + k * 32 + tid, x);
+    }
+  } else if (part == 0 && tid == 0 && a.logprob) {
+    const int col = token_col(load_id(a.tokens, a.token_bytes, row), a.r.V);
+    if (col >= 0) x_tok = T::to_f(x.p[col]);
+  }
+
+  Stat st{kNegInf, 0.0f, 0.0f};
+  // kTop: the table of maxima, a slot for every per_slot tiles
+  uint16_t* table = reinterpret_cast<uint16_t*>(mem);
+  const int tiles = (u_end - u_begin + kTile - 1) / kTile;
+  const int per_slot = (tiles + kSlots - 1) / kSlots;
+  int slot = 0, in_slot = 0;
+  uint32_t best[2] = {0, 0}, order = 0;
+
+  for (int u0 = u_begin; u0 < u_end; u0 += kTile) {
     Unit<T> w[T::kUnits];
-    float mx[T::kUnits];
+    load_tile<T, kThr>(x, u0, u_end, w);
+    float cm = unit_max<T>(w[0]);
 #pragma unroll
-    for (int u = 0; u < T::kUnits; ++u) {
-      const int i = u0 + u * kThreads + tid;
-      if (i < x.units)
-        w[u] = x.load(i);
-      else
-        w[u].w[0] = w[u].w[T::kWords - 1] = T::kWords == 1
-                                                ? make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u)
-                                                : make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
-    }
-#pragma unroll
-    for (int u = 0; u < T::kUnits; ++u) {
-      float v[8];
-      unpack<T>(w[u], v);
-      mx[u] = maxn(maxn(maxn(v[0], v[1]), maxn(v[2], v[3])), maxn(maxn(v[4], v[5]), maxn(v[6], v[7])));
-      fold8<kEnt>(v, mx[u], st, c2);
-    }
+    for (int u = 1; u < T::kUnits; ++u) cm = maxn(cm, unit_max<T>(w[u]));
+    fold_tile<T, kEnt>(w, cm, st, c2);
     if constexpr (kTop) {
-      // Columns grow from tile to tile and, inside a tile, from unit to unit.
-      if (u0 == 0) {
-        // tau = min over groups of threads of the group's largest unit maximum, with at least k groups:
-        // k elements of this tile are >= tau.  (fmaxf skips NaN maxima: the bound only gets lower.)
-        float g = kNegInf;
-#pragma unroll
-        for (int u = 0; u < T::kUnits; ++u) g = fmaxf(g, mx[u]);
-        int tpg = 32;
-        while (tpg > 1 && kThreads / tpg < a.k) tpg >>= 1;
-        for (int o = 1; o < tpg; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-        for (int o = tpg; o < 32; o <<= 1) g = fminf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-        if ((tid & 31) == 0) sh.tau[tid >> 5] = g;
-        __syncthreads();
-        tau = sh.tau[0];
-        for (int i = 1; i < kWarps; ++i) tau = fminf(tau, sh.tau[i]);
+      order = max(order, order16<T>(cm));
+      if (++in_slot == per_slot || u0 + kTile >= u_end) {
+        table[slot * kThr + tid] = static_cast<uint16_t>(order);
+        if (slot & 1)
+          best[1] = max(best[1], order);
+        else
+          best[0] = max(best[0], order);
+        ++slot;
+        in_slot = 0;
+        order = 0;
       }
-      auto append = [&](int u) {
-        bool high = false;
-        if (inclusive ? !(mx[u] < tau) : !(mx[u] <= tau)) {
-          float v[8];
-          unpack<T>(w[u], v);
-          const int c = x.col(u0 + u * kThreads + tid);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if ((inclusive ? !(v[j] < tau) : !(v[j] <= tau)) && c + j >= 0 && c + j < x.V) {
-              const int pos = atomicAdd(&sh.cnt, 1);
-              if (pos < kCand) keys[pos] = make_key<T>(v[j], static_cast<uint32_t>(c + j), a.ib);
-              high |= pos >= kCand / 2;
-            }
-          }
-        }
-        return high;
-      };
-      bool high = false;
-#pragma unroll
-      for (int u = 0; u < T::kUnits; ++u) high |= append(u);
-      if (__syncthreads_or(high)) {
-        int n = sh.cnt;
-        __syncthreads();
-        auto shrink = [&]() {
-          const uint64_t bound = keep_largest(keys, n, a.k, T::kKeyBits + a.ib, a.ib, sh);
-          n = a.k;
-          tau = key_value<T>(bound, a.ib);
-          inclusive = false;
-        };
-        if (n > kCand) {
-          // Too many for the buffer: drop this tile's keys and take its units one at a time, each
-          // of which (kSub columns) fits behind at most kCand - kSub keys.
-          n = filter_keys(keys, kCand, 0, x.col(u0) < 0 ? 0 : x.col(u0), a.ib, sh);
-#pragma unroll
-          for (int u = 0; u < T::kUnits; ++u) {
-            if (n > kCand - kSub) shrink();
-            append(u);
-            __syncthreads();
-            n = sh.cnt;
-            __syncthreads();
-          }
-        }
-        if (n > kCand / 2) shrink();
-      }
-      inclusive = false;  // later columns lose a tie
     }
   }
 
-  const Stat r = block_merge(st, sh_stat, c2);
-  const float l2 = log2f(r.s), ls = logf(r.s);
-  if constexpr (kDistill) {
-    if (tid < 32) {
-      float tm, tl;
-      const float loss = distill_row<T>(a, row, x, r.m, ls, &tm, &tl);
+  st = warp_merge(st, c2);
+  if ((tid & 31) == 0) sh_stat[warp] = st;
+  if constexpr (kTop) sh.maxima[tid] = best[0] | best[1] << 16;
+  __syncthreads();
+  if (warp == 0) {
+    st = tid < kNWarps ? sh_stat[tid] : Stat{kNegInf, 0.0f, 0.0f};
+    st = warp_merge(st, c2);
+    if constexpr (kTop) {
+      const uint32_t r = reached_by<kThr>(sh.maxima, a.k);
       if (tid == 0) {
-        a.loss[row] = loss;
-        if (a.stats) a.stats[row] = make_float4(r.m, l2, tm, tl);
+        sh.reached = r;
+        sh.items = sh.n = 0;
       }
     }
-    return;
-  } else {
-    if (tid == 0) {
-      const float H = kEnt ? __fmul_rn(kLn2, __fsub_rn(l2, __fdiv_rn(r.t, r.s))) : 0.0f;
-      if (a.logprob) {
-        const int col = token_col(load_id(a.tokens, a.token_bytes, row), a.r.V);
-        const float xv = col >= 0 ? T::to_f(x.p[col]) : __int_as_float(0x7FC00000);
-        a.logprob[row] = __fmaf_rn(__fsub_rn(xv, r.m), a.r.inv_t, -ls);
+  }
+  const uint64_t* mine = nullptr;
+  int n_mine = 0, n = 0;
+  const int bits = T::kKeyBits + a.ib;
+  if constexpr (kTop) {
+    __syncthreads();
+    n = find_top<T, kThr>(x, u_begin, u_end, per_slot, slot, a.k, a.ib, mem, sh, &mine, &n_mine);
+  }
+
+  if (n_parts > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    uint64_t* part_keys = reinterpret_cast<uint64_t*>(mem + TopLayout<kThr>::kBytes);  // [n_parts][cap]
+    if constexpr (kTop) {
+      if (n > a.cap) {
+        n = collect<kThr>(mine, n_mine, n, a.k, a.cap, bits, sh.last, sh);
+        const int per = (n + kNWarps - 1) / kNWarps;
+        mine = sh.last + warp * per;
+        n_mine = max(0, min(per, n - warp * per));
       }
-      if (a.entropy) a.entropy[row] = H;
-      if (a.stats) a.stats[row] = make_float4(r.m, l2, H, 0.0f);
+      if (tid == 0) sh.n = 0;
+      __syncthreads();
+    }
+    cluster.barrier_wait();
+    if constexpr (kTop) {
+      uint64_t* to = cluster.map_shared_rank(part_keys + part * a.cap, 0);
+      for (int i = tid & 31; i < n_mine; i += 32) to[atomicAdd(&sh.n, 1)] = mine[i];
+    }
+    if (tid == 0) {
+      PartsShared* to = cluster.map_shared_rank(&parts, 0);
+      to->stat[part] = st;
+      to->count[part] = n;
+    }
+    cluster.sync();
+    if (part > 0) return;
+    if (warp == 0) {
+      st = tid < n_parts ? parts.stat[tid] : Stat{kNegInf, 0.0f, 0.0f};
+      st = warp_merge(st, c2);
     }
     if constexpr (kTop) {
-      int n = sh.cnt;
-      __syncthreads();
-      if (n > a.k) keep_largest(keys, n, a.k, T::kKeyBits + a.ib, a.ib, sh);
-      n = a.k;  // V >= k: there are k
-      if (tid < n) {
-        const uint64_t key = keys[tid];
-        int rank = 0;
-        for (int i = 0; i < n; ++i) rank += keys[i] > key;
+      static_assert(kNWarps >= kMaxParts || kThr == 64, "a warp takes a part's keys");
+      mine = part_keys + warp * a.cap;
+      n_mine = warp < n_parts ? parts.count[warp] : 0;
+      n = 0;
+      for (int i = 0; i < n_parts; ++i) n += parts.count[i];
+    }
+  }
+
+  if (warp == 0) {
+    const float l2 = log2f(st.s), ls = logf(st.s);
+    if constexpr (kMode == kTeacher) {
+      float tm, tl;
+      const float loss = distill_row<T>(a, static_cast<int64_t>(row) * a.K, x, entry, st.m, ls, &tm, &tl);
+      if (tid == 0) {
+        a.loss[row] = loss;
+        if (a.stats) a.stats[row] = make_float4(st.m, l2, tm, tl);
+      }
+    } else if (tid == 0) {
+      const float H = kEnt ? __fmul_rn(kLn2, __fsub_rn(l2, __fdiv_rn(st.t, st.s))) : 0.0f;
+      if (a.logprob) a.logprob[row] = __fmaf_rn(__fsub_rn(x_tok, st.m), a.r.inv_t, -ls);
+      if (a.entropy) a.entropy[row] = H;
+      if (a.stats) a.stats[row] = make_float4(st.m, l2, H, 0.0f);
+      sh.m = st.m;
+      sh.ls = ls;
+    }
+  }
+  if constexpr (kTop) {
+    // V >= k: there are k keys at least
+    n = collect<kThr>(mine, n_mine, n, a.k, kFinal, bits, sh.last, sh);
+    const float m = sh.m, ls = sh.ls;
+    for (int i = tid; i < n; i += kThr) {
+      const uint64_t key = sh.last[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += sh.last[j] > key;
+      if (rank < a.k) {
         const uint32_t col = key_col(key, a.ib);
-        const float xv = T::to_f(x.p[col]);
-        a.top_lp[static_cast<int64_t>(row) * a.k + rank] = __fmaf_rn(__fsub_rn(xv, r.m), a.r.inv_t, -ls);
+        const float xv = T::kWords == 1 ? key_value<T>(key, a.ib) : T::to_f(x.p[col]);
+        a.top_lp[static_cast<int64_t>(row) * a.k + rank] = __fmaf_rn(__fsub_rn(xv, m), a.r.inv_t, -ls);
         a.top_id[static_cast<int64_t>(row) * a.k + rank] = col;
       }
     }
@@ -585,31 +914,6 @@ struct GradArgs {
   int tasks;     // tasks of a row
   int per_task;  // chunks of a task
 };
-
-// Two f32 at once (one issue slot of the FMA pipe for both).
-__device__ __forceinline__ uint64_t pk(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpk(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 
 // Entry j < n of a row: its column (-1: none) and the value that its weight comes from.
 template <bool kDistill>
@@ -831,18 +1135,46 @@ int check_out(const ufp8_logit_rows* x, int64_t outer, int64_t inner, const char
   return UFP8_OK;
 }
 
-template <class T, bool kEnt, bool kTop, bool kDistill>
-int launch_stat(const StatArgs& a, cudaStream_t s) {
-  const size_t smem = kTop ? sizeof(uint64_t) * kCand : 0;
-  rowstat_kernel<T, kEnt, kTop, kDistill><<<static_cast<unsigned>(a.r.rows), kThreads, smem, s>>>(a);
-  const cudaError_t e = cudaGetLastError();
+template <class T, int kThr, int kMode>
+int launch_stat(StatArgs& a, int part_bits, cudaStream_t s) {
+  a.part_bits = part_bits;
+  a.cap = 2 * a.k;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.r.rows << part_bits));
+  cfg.blockDim = dim3(kThr);
+  cfg.dynamicSmemBytes = kMode == kTopK ? TopLayout<kThr>::kBytes : 0;
+  if (kMode == kTopK && part_bits) cfg.dynamicSmemBytes += (sizeof(uint64_t) * a.cap) << part_bits;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 1u << part_bits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = part_bits ? 1 : 0;
+  static thread_local int smem_dev = -1;  // more than 48 KB of dynamic shared memory is asked for once per device
+  int cur = 0;
+  cudaError_t e = cudaGetDevice(&cur);
+  if (e == cudaSuccess && kMode == kTopK && smem_dev != cur) {
+    e = cudaFuncSetAttribute(rowstat_kernel<T, kThr, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(TopLayout<kThr>::kBytes + sizeof(uint64_t) * 2 * kMaxTop * kMaxParts));
+    smem_dev = cur;
+  }
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, rowstat_kernel<T, kThr, kMode>, a);
   return e == cudaSuccess ? UFP8_OK : cuda_error(e, "row statistics launch");
 }
 
-template <class T>
-int launch_logprob(const StatArgs& a, bool ent, cudaStream_t s) {
-  if (a.k > 0) return ent ? launch_stat<T, true, true, false>(a, s) : launch_stat<T, false, true, false>(a, s);
-  return ent ? launch_stat<T, true, false, false>(a, s) : launch_stat<T, false, false, false>(a, s);
+template <class T, int kMode>
+int launch_stat(StatArgs& a, cudaStream_t s) {
+  constexpr int kTile = 256 * T::kUnits * 8;  // columns
+  // few rows: a row is split as long as its parts are whole tiles and the rows alone do not fill the device
+  int bits = 0;
+  while (bits < 3 && (a.r.rows << bits) < 296 && (static_cast<int64_t>(a.r.V) >> bits) > kTile) ++bits;
+  return launch_stat<T, 256, kMode>(a, bits, s);
+}
+
+template <int kMode>
+int launch_stat(StatArgs& a, int dtype, cudaStream_t s) {
+  return dtype == UFP8_OUT_F32 ? launch_stat<F32, kMode>(a, s) : launch_stat<Bf16, kMode>(a, s);
 }
 
 template <class T, bool kDistill>
@@ -906,9 +1238,9 @@ extern "C" int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens
   a.top_lp = top_logprobs;
   a.top_id = top_ids;
   a.stats = reinterpret_cast<float4*>(stats);
-  const bool ent = entropy != nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return x->dtype == UFP8_OUT_F32 ? launch_logprob<F32>(a, ent, s) : launch_logprob<Bf16>(a, ent, s);
+  if (top_k > 0) return launch_stat<kTopK>(a, x->dtype, s);
+  return entropy ? launch_stat<kEntropy>(a, x->dtype, s) : launch_stat<kPlain>(a, x->dtype, s);
 }
 
 extern "C" int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const void* tokens,
@@ -985,8 +1317,7 @@ extern "C" int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teache
   a.loss = loss;
   a.stats = reinterpret_cast<float4*>(stats);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return x->dtype == UFP8_OUT_F32 ? launch_stat<F32, false, false, true>(a, s)
-                                  : launch_stat<Bf16, false, false, true>(a, s);
+  return launch_stat<kTeacher>(a, x->dtype, s);
 }
 
 extern "C" int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stats, const void* teacher_ids,
