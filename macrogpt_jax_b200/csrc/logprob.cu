@@ -320,7 +320,7 @@ constexpr int kMaxParts = 8;  // CTAs of a cluster that share a row
 template <int kThr>
 struct TopLayout {
   static constexpr int kItems = 4 * kThr;
-  static constexpr int kGather = kThr == 256 ? 1024 : 512;
+  static constexpr int kGather = kThr >= 128 ? 1024 : 512;
   static constexpr size_t kTableBytes = sizeof(uint16_t) * kSlots * kThr;
   static constexpr size_t kItemBytes = sizeof(uint32_t) * kItems;
   static constexpr size_t kFast = kTableBytes + kItemBytes + sizeof(uint64_t) * kGather;
@@ -359,9 +359,21 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t* maxima, int k) {
     hi[i] = w >> 16;
     if (!halves) lo[i] = max(lo[i], hi[i]);
   }
-  uint32_t b = 0;
+  if (k > kThr * (halves ? 2 : 1)) return 0;
+  // the bits that all have in common need no counting
+  uint32_t mn = lo[0], mx = lo[0];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    mn = min(mn, halves ? min(lo[i], hi[i]) : lo[i]);
+    mx = max(mx, halves ? max(lo[i], hi[i]) : lo[i]);
+  }
+  mn = __reduce_min_sync(0xFFFFFFFFu, mn);
+  mx = __reduce_max_sync(0xFFFFFFFFu, mx);
+  if (mn == mx) return mx;
+  uint32_t bit = 0x80000000u >> __clz(mn ^ mx);
+  uint32_t b = mx & ~(2 * bit - 1);
 #pragma unroll 1
-  for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+  for (; bit; bit >>= 1) {
     const uint32_t c = b | bit;
     int cnt = 0;
 #pragma unroll
@@ -615,6 +627,21 @@ __device__ __forceinline__ void load_tile(const Row<T>& x, int u0, int u_end, Un
   }
 }
 
+// The warp's candidates among the CTA's units [u_begin, u_end), into its region; returns their number.
+template <class T, int kThr>
+__device__ __noinline__ int search_row(const Row<T>& x, int u_begin, int u_end, int k, int ib, uint32_t reached,
+                                       uint64_t* region) {
+  Search<T> top(region, k, ib, reached);
+  for (int u0 = u_begin; u0 < u_end; u0 += kThr * T::kUnits) {
+    Unit<T> w[T::kUnits];
+    load_tile<T, kThr>(x, u0, u_end, w);
+#pragma unroll
+    for (int u = 0; u < T::kUnits; ++u)
+      top.take(w[u], unit_max<T>(w[u]), x.col(u0 + u * kThr + threadIdx.x), x.V);
+  }
+  return top.n;
+}
+
 // The k largest of the CTA's units [u_begin, u_end), and a few more, as keys: this warp's list (*mine, *n_mine);
 // returns the number of all warps.  `reached` is a bound that k of the elements reach.  Its table says which
 // thread and which tiles saw a maximum that reaches it; those (little more than k) are read once more.
@@ -673,19 +700,12 @@ __device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end,
     return n;
   }
   __syncthreads();  // the table, the items and the gathered keys give way to the regions
-  Search<T> top(reinterpret_cast<uint64_t*>(mem) + warp * kRegion, k, ib, reached);
+  uint64_t* region = reinterpret_cast<uint64_t*>(mem) + warp * kRegion;
+  *mine = region;
+  *n_mine = search_row<T, kThr>(x, u_begin, u_end, k, ib, reached, region);
   if (tid == 0) sh.n = 0;
-  for (int u0 = u_begin; u0 < u_end; u0 += kTile) {
-    Unit<T> w[T::kUnits];
-    load_tile<T, kThr>(x, u0, u_end, w);
-#pragma unroll
-    for (int u = 0; u < T::kUnits; ++u)
-      top.take(w[u], unit_max<T>(w[u]), x.col(u0 + u * kThr + tid), x.V);
-  }
-  *mine = top.keys;
-  *n_mine = top.n;
   __syncthreads();
-  if ((tid & 31) == 0) atomicAdd(&sh.n, top.n);
+  if ((tid & 31) == 0) atomicAdd(&sh.n, *n_mine);
   __syncthreads();
   return sh.n;
 }
@@ -707,7 +727,7 @@ __device__ __forceinline__ int collect(const uint64_t* mine, int n_mine, int n, 
 
 // One CTA per row, or a cluster of 2 to 8 that share a row's units and bring their parts to the first of them.
 template <class T, int kThr, int kMode>
-__global__ void __launch_bounds__(kThr) rowstat_kernel(const StatArgs a) {
+__global__ void __launch_bounds__(kThr, (kMode == kTopK ? 4 : 6) * 256 / kThr) rowstat_kernel(const StatArgs a) {
   constexpr bool kEnt = kMode == kEntropy || kMode == kTopK;
   constexpr bool kTop = kMode == kTopK;
   constexpr int kNWarps = kThr / 32;
@@ -843,7 +863,7 @@ __global__ void __launch_bounds__(kThr) rowstat_kernel(const StatArgs a) {
       st = warp_merge(st, c2);
     }
     if constexpr (kTop) {
-      static_assert(kNWarps >= kMaxParts || kThr == 64, "a warp takes a part's keys");
+      static_assert(kNWarps >= kMaxParts || kThr < 256, "a warp takes a part's keys");
       mine = part_keys + warp * a.cap;
       n_mine = warp < n_parts ? parts.count[warp] : 0;
       n = 0;
@@ -870,13 +890,19 @@ __global__ void __launch_bounds__(kThr) rowstat_kernel(const StatArgs a) {
     }
   }
   if constexpr (kTop) {
-    // V >= k: there are k keys at least
-    n = collect<kThr>(mine, n_mine, n, a.k, kFinal, bits, sh.last, sh);
+    // V >= k: there are k keys at least.  The keys of one CTA that are not many lie one after another.
+    const uint64_t* last = mine - warp * ((n + kNWarps - 1) / kNWarps);
+    if (n_parts > 1 || n > kFinal) {
+      n = collect<kThr>(mine, n_mine, n, a.k, kFinal, bits, sh.last, sh);
+      last = sh.last;
+    } else {
+      __syncthreads();  // sh.m, sh.ls
+    }
     const float m = sh.m, ls = sh.ls;
     for (int i = tid; i < n; i += kThr) {
-      const uint64_t key = sh.last[i];
+      const uint64_t key = last[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += sh.last[j] > key;
+      for (int j = 0; j < n; ++j) rank += last[j] > key;
       if (rank < a.k) {
         const uint32_t col = key_col(key, a.ib);
         const float xv = T::kWords == 1 ? key_value<T>(key, a.ib) : T::to_f(x.p[col]);
@@ -1166,9 +1192,16 @@ int launch_stat(StatArgs& a, int part_bits, cudaStream_t s) {
 template <class T, int kMode>
 int launch_stat(StatArgs& a, cudaStream_t s) {
   constexpr int kTile = 256 * T::kUnits * 8;  // columns
-  // few rows: a row is split as long as its parts are whole tiles and the rows alone do not fill the device
+  // Few rows: a row is split as long as its parts are whole tiles and all CTAs run at once (those that
+  // search for alternatives take more of an SM).
+  const int64_t most = kMode == kTopK ? 400 : 800;
   int bits = 0;
-  while (bits < 3 && (a.r.rows << bits) < 296 && (static_cast<int64_t>(a.r.V) >> bits) > kTile) ++bits;
+  while (bits < 3 && (a.r.rows << (bits + 1)) <= most && (static_cast<int64_t>(a.r.V) >> bits) > kTile) ++bits;
+  // Many short rows: smaller CTAs, more of which are resident, hide each other's ends.
+  if (a.r.rows >= 592) {
+    if (a.r.V <= 8192 && a.k <= 64) return launch_stat<T, 64, kMode>(a, 0, s);
+    if (a.r.V <= (kMode == kTopK ? 32768 : 16384) && a.k <= 128) return launch_stat<T, 128, kMode>(a, 0, s);
+  }
   return launch_stat<T, 256, kMode>(a, bits, s);
 }
 

@@ -22,16 +22,16 @@ MAX_ENTRIES = 1024
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, mask, temperature):
-        loss, stats = ops.distill_forward(ops.logit_rows(logits), ids, teacher, mask, temperature, True)
+        loss, stats = ops.distill_forward(logits, ids, teacher, mask, temperature, True)
         ctx.save_for_backward(logits, ids, teacher, mask, stats)
         ctx.temperature = temperature
-        return loss.view(logits.shape[:-1])
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         logits, ids, teacher, mask, stats = ctx.saved_tensors
-        dlogits = ops.distill_backward(ops.logit_rows(logits), stats, ids, teacher, mask, ctx.temperature, dloss)
+        dlogits = ops.distill_backward(logits, stats, ids, teacher, mask, ctx.temperature, dloss)
         return dlogits, None, None, None, None
 
 
@@ -54,7 +54,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
         raise ValueError(f"{who}: teacher_ids {tuple(teacher_ids.shape)}: at most {MAX_ENTRIES} entries per row")
     shape = (*logits.shape[:-1], teacher_ids.shape[-1])
     ids = check_ids(teacher_ids, shape, logits, "teacher_ids", who)
-    if tuple(teacher_logits.shape) != shape or teacher_logits.device != logits.device:
+    if teacher_logits.shape != shape or teacher_logits.device != logits.device:
         raise ValueError(f"{who}: teacher_logits {tuple(teacher_logits.shape)} on {teacher_logits.device}, expected "
                          f"{shape} on {logits.device}")
     if teacher_logits.dtype not in (torch.bfloat16, torch.float32):
@@ -65,5 +65,4 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     mask = check_mask(mask, logits, who)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillFn.apply(logits, ids, teacher, mask, temperature)
-    loss, _ = ops.distill_forward(ops.logit_rows(logits), ids, teacher, mask, temperature, False)
-    return loss.view(logits.shape[:-1])
+    return ops.distill_forward(logits, ids, teacher, mask, temperature, False)[0]

@@ -60,7 +60,7 @@ def check_mask(mask: Optional[torch.Tensor], logits: torch.Tensor, who: str) -> 
 
 def check_ids(ids: torch.Tensor, shape, logits: torch.Tensor, name: str, who: str) -> torch.Tensor:
     """Contiguous int32 or int64 ids of the given shape on the logits' device."""
-    if tuple(ids.shape) != tuple(shape) or ids.device != logits.device:
+    if ids.shape != shape or ids.device != logits.device:
         raise ValueError(f"{who}: {name} {tuple(ids.shape)} on {ids.device}, expected {tuple(shape)} on "
                          f"{logits.device}")
     if ids.dtype not in (torch.int32, torch.int64):
@@ -73,18 +73,13 @@ def check_ids(ids: torch.Tensor, shape, logits: torch.Tensor, name: str, who: st
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, mask, top_k, temperature, entropy):
-        lr = ops.logit_rows(logits)
-        lead = logits.shape[:-1]
-        lp, ent, top_lp, top_id, stats = ops.token_logprobs_forward(lr, tokens, mask, top_k, temperature, entropy, True)
-        out = tuple(None if t is None else t.view(s) for t, s in
-                    ((lp, lead), (ent, lead), (top_lp, (*lead, top_k)), (top_id, (*lead, top_k))))
-        if top_id is not None:
+        out = ops.token_logprobs_forward(logits, tokens, mask, top_k, temperature, entropy, True)
+        if top_k:
             ctx.mark_non_differentiable(out[3])
         ctx.set_materialize_grads(False)
-        # the rows are taken again in the backward: the saved tensor may be unpacked as another one
-        ctx.save_for_backward(logits, tokens, mask, stats, out[3])
+        ctx.save_for_backward(logits, tokens, mask, out[4], out[3])
         ctx.temperature = temperature
-        return out
+        return out[:4]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -92,8 +87,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
         logits, tokens, mask, stats, top_id = ctx.saved_tensors
         if dlp is None and dent is None and dtop is None:
             return None, None, None, None, None, None
-        dlogits = ops.token_logprobs_backward(ops.logit_rows(logits), stats, tokens, mask, ctx.temperature, dlp, dent,
-                                              dtop, top_id)
+        dlogits = ops.token_logprobs_backward(logits, stats, tokens, mask, ctx.temperature, dlp, dent, dtop, top_id)
         return dlogits, None, None, None, None, None
 
 
@@ -124,8 +118,4 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     mask = check_mask(mask, logits, who)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, tokens, mask, top_k, temperature, entropy))
-    lp, ent, top_lp, top_id, _ = ops.token_logprobs_forward(ops.logit_rows(logits), tokens, mask, top_k, temperature,
-                                                            entropy, False)
-    return TokenLogprobs(None if lp is None else lp.view(lead), None if ent is None else ent.view(lead),
-                         None if top_lp is None else top_lp.view(*lead, top_k),
-                         None if top_id is None else top_id.view(*lead, top_k))
+    return TokenLogprobs(*ops.token_logprobs_forward(logits, tokens, mask, top_k, temperature, entropy, False)[:4])

@@ -7,6 +7,7 @@ no CPU path: inputs must be CUDA tensors and a missing library raises.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -524,8 +525,7 @@ def head_xent_backward(dloss: torch.Tensor, saved, labels: torch.Tensor, mask: t
 _LOGIT_DTYPE = {torch.bfloat16: C.OUT_BF16, torch.float32: C.OUT_F32}
 
 
-@dataclass(frozen=True)
-class LogitRows:
+class LogitRows(NamedTuple):
     """The rows of a logits tensor [..., V] as the kernels address them (include/ufp8.h).  `logits` is
     the tensor itself, or a contiguous copy where its strides have more than two levels."""
     logits: torch.Tensor
@@ -537,7 +537,21 @@ class LogitRows:
     def c(self, temperature: float, mask: torch.Tensor | None) -> C.LogitRows:
         t = self.logits
         return C.LogitRows(t.data_ptr(), _LOGIT_DTYPE[t.dtype], temperature, self.rows, t.shape[-1], self.inner,
-                           self.stride_outer, self.stride_inner, mask.data_ptr() if mask is not None else None)
+                           self.stride_outer, self.stride_inner, _ptr(mask))
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _launch_on(device: torch.device, kind: str, work: float, fn) -> None:
+    """fn(stream) on the current stream of `device`, which may be another one than the current device."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        _launch(kind, work, lambda: fn(torch.cuda.current_stream(index).cuda_stream))
+    else:
+        with torch.cuda.device(index):
+            _launch(kind, work, lambda: fn(torch.cuda.current_stream(index).cuda_stream))
 
 
 def logit_rows(logits: torch.Tensor) -> LogitRows:
@@ -567,34 +581,32 @@ def _grad_rows(lr: LogitRows):
     16-byte boundary; otherwise each row starts as far from such a boundary as its logit row (the
     backward then loads and stores 16 bytes at a time), by a few elements between the rows."""
     t = lr.logits
-    V, e = t.shape[-1], 16 // t.element_size()
-    start = (t.data_ptr() // t.element_size()) % e
-    inner = V + (lr.stride_inner - V) % e
-    outer = lr.inner * inner + (lr.stride_outer - lr.inner * inner) % e if lr.rows > lr.inner else lr.inner * inner
+    V, es = t.shape[-1], t.element_size()
+    e = 16 // es
+    start = (t.data_ptr() // es) % e
     if start == 0 and t.is_contiguous():
         return torch.empty_like(t), 0, V
+    inner = V + (lr.stride_inner - V) % e
+    outer = lr.inner * inner + (lr.stride_outer - lr.inner * inner) % e if lr.rows > lr.inner else lr.inner * inner
     n_outer = lr.rows // lr.inner
     buf = torch.empty(start + n_outer * outer, dtype=t.dtype, device=t.device)
     return buf.as_strided((n_outer, lr.inner, V), (outer, inner, 1), start).view(t.shape), outer, inner
 
 
-def token_logprobs_forward(lr: LogitRows, tokens: torch.Tensor | None, mask: torch.Tensor | None, top_k: int,
+def token_logprobs_forward(logits: torch.Tensor, tokens: torch.Tensor | None, mask: torch.Tensor | None, top_k: int,
                            temperature: float, entropy: bool, want_stats: bool):
-    """(logprob, entropy, top log probabilities, top ids, stats) over the flattened rows; None where not
-    asked for (ufp8_logprob_forward)."""
-    t, rows = lr.logits, lr.rows
-    dev, V = t.device, t.shape[-1]
-    f32 = {"dtype": torch.float32, "device": dev}
-    lp = torch.empty(rows, **f32) if tokens is not None else None
-    ent = torch.empty(rows, **f32) if entropy else None
-    top_lp = torch.empty((rows, top_k), **f32) if top_k else None
-    top_id = torch.empty((rows, top_k), dtype=torch.int64, device=dev) if top_k else None
-    stats = torch.empty((rows, 4), **f32) if want_stats else None
-    ptr = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
-    with torch.cuda.device(dev):
-        _launch("logprob", float(t.element_size()) * rows * V, lambda: C.logprob_forward(
-            lr.c(temperature, mask), ptr(tokens), tokens.element_size() if tokens is not None else 0, top_k, ptr(lp),
-            ptr(ent), ptr(top_lp), ptr(top_id), ptr(stats), _stream()))
+    """(logprob, entropy, top log probabilities, top ids) over the logits' leading shape, then the
+    backward's stats; None where not asked for (ufp8_logprob_forward)."""
+    lr = logit_rows(logits)
+    t, lead, dev, f32 = lr.logits, logits.shape[:-1], logits.device, torch.float32
+    lp = torch.empty(lead, dtype=f32, device=dev) if tokens is not None else None
+    ent = torch.empty(lead, dtype=f32, device=dev) if entropy else None
+    top_lp = torch.empty((*lead, top_k), dtype=f32, device=dev) if top_k else None
+    top_id = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
+    stats = torch.empty((lr.rows, 4), dtype=f32, device=dev) if want_stats else None
+    _launch_on(dev, "logprob", float(t.element_size()) * t.numel(), lambda stream: C.logprob_forward(
+        lr.c(temperature, mask), _ptr(tokens), tokens.element_size() if tokens is not None else 0, top_k, _ptr(lp),
+        _ptr(ent), _ptr(top_lp), _ptr(top_id), _ptr(stats), stream))
     return lp, ent, top_lp, top_id, stats
 
 
@@ -603,55 +615,54 @@ def _row_grad(g: torch.Tensor | None):
     expanded over the rows (what .sum() and .mean() send back)."""
     if g is None:
         return None, 0
-    g = g.to(torch.float32)
-    if not any(g.stride()):
-        return g, 0
-    return g.contiguous(), 1
+    if g.dtype != torch.float32:
+        g = g.to(torch.float32)
+    if g.is_contiguous():
+        return g, 1
+    return (g.contiguous(), 1) if any(g.stride()) else (g, 0)
 
 
-def token_logprobs_backward(lr: LogitRows, stats: torch.Tensor, tokens: torch.Tensor | None, mask: torch.Tensor | None,
-                            temperature: float, dlp: torch.Tensor | None, dent: torch.Tensor | None,
-                            dtop: torch.Tensor | None, top_id: torch.Tensor | None) -> torch.Tensor:
+def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: torch.Tensor | None,
+                            mask: torch.Tensor | None, temperature: float, dlp: torch.Tensor | None,
+                            dent: torch.Tensor | None, dtop: torch.Tensor | None,
+                            top_id: torch.Tensor | None) -> torch.Tensor:
     """dlogits of token_logprobs_forward (ufp8_logprob_backward)."""
-    t, rows = lr.logits, lr.rows
+    lr = logit_rows(logits)
+    t = lr.logits
     dlp, s_lp = _row_grad(dlp)
     dent, s_ent = _row_grad(dent)
     dtop = None if dtop is None else dtop.to(torch.float32).contiguous()
     top_k = top_id.shape[-1] if dtop is not None else 0
-    ptr = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
-    with torch.cuda.device(t.device):
-        out, outer, inner = _grad_rows(lr)
-        _launch("logprob_grad", 2.0 * t.element_size() * rows * t.shape[-1], lambda: C.logprob_backward(
-            lr.c(temperature, mask), stats.data_ptr(), ptr(tokens), tokens.element_size() if tokens is not None else 0,
-            ptr(dlp), s_lp, ptr(dent), s_ent, ptr(dtop), ptr(top_id), top_k, out.data_ptr(), outer, inner, _stream()))
+    out, outer, inner = _grad_rows(lr)
+    _launch_on(t.device, "logprob_grad", 2.0 * t.element_size() * t.numel(), lambda stream: C.logprob_backward(
+        lr.c(temperature, mask), stats.data_ptr(), _ptr(tokens), tokens.element_size() if tokens is not None else 0,
+        _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, out.data_ptr(), outer, inner, stream))
     return out
 
 
-def distill_forward(lr: LogitRows, ids: torch.Tensor, teacher: torch.Tensor, mask: torch.Tensor | None,
+def distill_forward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, mask: torch.Tensor | None,
                     temperature: float, want_stats: bool):
-    """(loss, stats) over the flattened rows (ufp8_distill_forward)."""
-    t, rows = lr.logits, lr.rows
-    loss = torch.empty(rows, dtype=torch.float32, device=t.device)
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=t.device) if want_stats else None
-    with torch.cuda.device(t.device):
-        _launch("distill", float(t.element_size()) * rows * t.shape[-1], lambda: C.distill_forward(
-            lr.c(temperature, mask), ids.data_ptr(), ids.element_size(), teacher.data_ptr(),
-            _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], loss.data_ptr(),
-            stats.data_ptr() if stats is not None else None, _stream()))
+    """(loss over the logits' leading shape, the backward's stats) (ufp8_distill_forward)."""
+    lr = logit_rows(logits)
+    t = lr.logits
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=t.device)
+    stats = torch.empty((lr.rows, 4), dtype=torch.float32, device=t.device) if want_stats else None
+    _launch_on(t.device, "distill", float(t.element_size()) * t.numel(), lambda stream: C.distill_forward(
+        lr.c(temperature, mask), ids.data_ptr(), ids.element_size(), teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype],
+        ids.shape[-1], loss.data_ptr(), _ptr(stats), stream))
     return loss, stats
 
 
-def distill_backward(lr: LogitRows, stats: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
+def distill_backward(logits: torch.Tensor, stats: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
                      mask: torch.Tensor | None, temperature: float, dloss: torch.Tensor) -> torch.Tensor:
     """dlogits of distill_forward (ufp8_distill_backward)."""
-    t, rows = lr.logits, lr.rows
+    lr = logit_rows(logits)
+    t = lr.logits
     dloss, stride = _row_grad(dloss)
-    with torch.cuda.device(t.device):
-        out, outer, inner = _grad_rows(lr)
-        _launch("distill_grad", 2.0 * t.element_size() * rows * t.shape[-1], lambda: C.distill_backward(
-            lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(), ids.element_size(), teacher.data_ptr(),
-            _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride, out.data_ptr(), outer, inner,
-            _stream()))
+    out, outer, inner = _grad_rows(lr)
+    _launch_on(t.device, "distill_grad", 2.0 * t.element_size() * t.numel(), lambda stream: C.distill_backward(
+        lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(), ids.element_size(), teacher.data_ptr(),
+        _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride, out.data_ptr(), outer, inner, stream))
     return out
 
 
