@@ -93,6 +93,20 @@ __device__ __forceinline__ void unpack(const Unit<T>& u, float (&v)[8]) {
   }
 }
 
+// Element j of a unit, j not known at compile time.
+template <class T>
+__device__ __forceinline__ float pick(const Unit<T>& u, int j) {
+  if constexpr (T::kWords == 1) {
+    const uint32_t lo = (j & 2) ? u.w[0].y : u.w[0].x, hi = (j & 2) ? u.w[0].w : u.w[0].z;
+    const uint32_t w = (j & 4) ? hi : lo;
+    return __uint_as_float((j & 1) ? w & 0xFFFF0000u : w << 16);
+  } else {
+    const uint4 w = (j & 4) ? u.w[1] : u.w[0];
+    const uint32_t a = (j & 1) ? w.y : w.x, b = (j & 1) ? w.w : w.z;
+    return __uint_as_float((j & 2) ? b : a);
+  }
+}
+
 // A row as units of 8 elements that start on 16-byte boundaries: unit i covers the columns
 // [8 i - off, 8 i - off + 8) where off elements lie between the boundary at or below the row's first
 // element and that element.  Only the first and the last unit can reach outside the row; those read
@@ -333,16 +347,17 @@ struct TopShared {
   uint32_t hist[256];
   uint32_t maxima[kThr];  // order16 of a thread's maximum over the even / odd slots of the table
   uint32_t reached;       // order16 that at least k elements of the CTA's columns reach (0: not known)
-  int items, n;
+  int items, n, n_last;   // entries of the item list, gathered keys, keys in `last`
   int bin, above, in_bin;
-  uint64_t last[kFinal];
   float m, ls;
+  alignas(16) uint64_t last[kFinal];
 };
 
 // What the CTAs of a cluster bring to the first one of it.
 struct PartsShared {
   Stat stat[kMaxParts];
   int count[kMaxParts];
+  uint32_t reached[kMaxParts];
 };
 
 // The largest 16-bit order that at least k of the maxima reach, found bit by bit by one warp; 0 where there
@@ -471,6 +486,19 @@ __device__ uint64_t select_bound(const uint64_t* mine, int n_mine, int k, int bi
   return bound;
 }
 
+// Bit j: element j of the unit at columns c ... c + 7 lies in the row and is not <= thr.
+template <class T>
+__device__ __forceinline__ unsigned above(const Unit<T>& w, float thr, int c, int V) {
+  float v[8];
+  unpack<T>(w, v);
+  unsigned hit = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) hit |= !(v[j] <= thr) ? 1u << j : 0u;
+  if (c < 0) hit &= 0xFFu << min(-c, 8);
+  if (c + 8 > V) hit &= 0xFFu >> min(c + 8 - V, 8);
+  return hit;
+}
+
 // A warp's search of a whole row for candidates, for rows with more elements at the bound than fit.  An
 // element is a candidate if it is above `thr`, below which k elements of the row lie: either those that
 // `reached` vouches for (equal elements included, since those k may stand further right), or k of the
@@ -485,15 +513,7 @@ struct Search {
       : keys(region), k(k_), ib(ib_), thr(below_order(reached)) {}
   // unit: 8 columns from c on for every lane, right of all columns before
   __device__ __forceinline__ void take(const Unit<T>& unit, float mx, int c, int V) {
-    unsigned hit = 0;
-    if (!(mx <= thr)) {
-      float v[8];
-      unpack<T>(unit, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) hit |= !(v[j] <= thr) ? 1u << j : 0u;
-      if (c < 0) hit &= 0xFFu << min(-c, 8);
-      if (c + 8 > V) hit &= 0xFFu >> min(c + 8 - V, 8);
-    }
+    unsigned hit = !(mx <= thr) ? above<T>(unit, thr, c, V) : 0;
     unsigned who = __ballot_sync(0xFFFFFFFFu, hit != 0);
     if (who == 0) return;
     if (n > kRegion - 256) {
@@ -506,11 +526,7 @@ struct Search {
       if (hit) {
         const int j = __ffs(hit) - 1;
         hit &= hit - 1;
-        float v[8];
-        unpack<T>(unit, v);
-        float x = v[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) x = i == j ? v[i] : x;
+        const float x = pick<T>(unit, j);
         keys[n + __popc(who & ((1u << lane) - 1u))] = make_key<T>(x, static_cast<uint32_t>(c + j), ib);
       }
       n += __popc(who);
@@ -643,50 +659,69 @@ __device__ __noinline__ int search_row(const Row<T>& x, int u_begin, int u_end, 
 }
 
 // The k largest of the CTA's units [u_begin, u_end), and a few more, as keys: this warp's list (*mine, *n_mine);
-// returns the number of all warps.  `reached` is a bound that k of the elements reach.  Its table says which
-// thread and which tiles saw a maximum that reaches it; those (little more than k) are read once more.
-// Where too many elements equal the bound (a constant row, say), the row is searched as a whole.
+// returns the number of all warps.  `reached` is a bound that k of the elements reach, `best` the thread's
+// maximum.  The table says which thread and which tiles saw a maximum that reaches it; those (little more
+// than k) are read once more, each by one thread.  Where too many elements equal the bound (a constant
+// row, say), the row is searched as a whole.
 template <class T, int kThr>
-__device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end, int per_slot, int slots, int k, int ib,
-                                        char* mem, TopShared<kThr>& sh, const uint64_t** mine, int* n_mine) {
+__device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end, int per_slot, int slots, uint32_t best,
+                                        int k, int ib, char* mem, TopShared<kThr>& sh, const uint64_t** mine,
+                                        int* n_mine) {
   using L = TopLayout<kThr>;
   constexpr int kTile = kThr * T::kUnits;
-  const int tid = threadIdx.x, warp = tid >> 5;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint16_t* table = reinterpret_cast<const uint16_t*>(mem);
   uint32_t* items = reinterpret_cast<uint32_t*>(mem + L::kTableBytes);
   uint64_t* gather = reinterpret_cast<uint64_t*>(mem + L::kTableBytes + L::kItemBytes);
   const uint32_t reached = sh.reached;
   const float thr = below_order(reached);
-  for (int slot = 0; slot < slots; ++slot)
-    if (table[slot * kThr + tid] >= reached) {
-      const int at = atomicAdd(&sh.items, 1);
-      if (at < L::kItems) items[at] = static_cast<uint32_t>(slot << 16 | tid);
+  if (__any_sync(0xFFFFFFFFu, best >= reached)) {
+    unsigned hits = 0;  // the lane's slots; kSlots <= 32
+#pragma unroll 4
+    for (int slot = 0; slot < slots; ++slot)
+      hits |= table[slot * kThr + tid] >= reached ? 1u << slot : 0u;
+    const int mine_n = __popc(hits);
+    int before = mine_n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xFFFFFFFFu, before, o);
+      if (lane >= o) before += up;
     }
+    int at = 0;
+    if (lane == 31) at = atomicAdd(&sh.items, before);
+    at = __shfl_sync(0xFFFFFFFFu, at, 31) + before - mine_n;
+    for (; hits; hits &= hits - 1, ++at)
+      if (at < L::kItems) items[at] = static_cast<uint32_t>((__ffs(hits) - 1) << 16 | tid);
+  }
   __syncthreads();
   const int m = sh.items;
   if (m <= L::kItems) {
-    for (int it = tid; it < m; it += kThr) {
-      const int slot = items[it] >> 16, t = items[it] & 0xFFFFu;
-      for (int tile = slot * per_slot; tile < (slot + 1) * per_slot; ++tile) {
-        Unit<T> w[T::kUnits];
+    constexpr int kFlight = 2;  // units per thread whose loads are in flight together
+#pragma unroll 1
+    for (int q0 = tid; q0 < m * T::kUnits; q0 += kFlight * kThr) {
+#pragma unroll 1
+      for (int tile = 0; tile < per_slot; ++tile) {
+        Unit<T> w[kFlight];
+        int i[kFlight];
 #pragma unroll
-        for (int u = 0; u < T::kUnits; ++u) {
-          const int i = u_begin + tile * kTile + u * kThr + t;
-          if (i < u_end) w[u] = x.load(i);
+        for (int f = 0; f < kFlight; ++f) {
+          const int q = q0 + f * kThr;
+          i[f] = u_end;
+          if (q < m * T::kUnits) {
+            const uint32_t item = items[q / T::kUnits];
+            i[f] = u_begin + (static_cast<int>(item >> 16) * per_slot + tile) * kTile + q % T::kUnits * kThr +
+                   (item & 0xFFFFu);
+            if (i[f] < u_end) w[f] = x.load(i[f]);
+          }
         }
 #pragma unroll
-        for (int u = 0; u < T::kUnits; ++u) {
-          const int i = u_begin + tile * kTile + u * kThr + t;
-          if (i >= u_end || unit_max<T>(w[u]) <= thr) continue;
-          float v[8];
-          unpack<T>(w[u], v);
-          const int c = x.col(i);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(v[j] <= thr) && c + j >= 0 && c + j < x.V) {
-              const int at = atomicAdd(&sh.n, 1);
-              if (at < L::kGather) gather[at] = make_key<T>(v[j], static_cast<uint32_t>(c + j), ib);
-            }
+        for (int f = 0; f < kFlight; ++f) {
+          if (i[f] >= u_end) continue;
+          for (unsigned hit = above<T>(w[f], thr, x.col(i[f]), x.V); hit; hit &= hit - 1) {
+            const int j = __ffs(hit) - 1;
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < L::kGather) gather[at] = make_key<T>(pick<T>(w[f], j), static_cast<uint32_t>(x.col(i[f]) + j), ib);
+          }
         }
       }
     }
@@ -710,24 +745,36 @@ __device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end,
   return sh.n;
 }
 
-// The warps' lists, cut to exactly k keys if they hold more than `most` (>= k, <= room of out), into out in any order;
-// returns their number.  Whole CTA; begins and ends with a barrier.
+// Those >= bound of the n keys in the warps' lists (k of them at least), cut to exactly k if there are more than
+// `most` (>= k), into sh.last in any order; returns their number.  sh.n_last is 0 before.  Whole CTA; ends with a
+// barrier.
 template <int kThr>
-__device__ __forceinline__ int collect(const uint64_t* mine, int n_mine, int n, int k, int most, int bits,
-                                       uint64_t* out, TopShared<kThr>& sh) {
-  const uint64_t bound = n > most ? select_bound<kThr>(mine, n_mine, k, bits, sh) : 0;
+__device__ __forceinline__ int collect(const uint64_t* mine, int n_mine, int n, int k, int most, uint64_t bound,
+                                       int bits, TopShared<kThr>& sh) {
+  const int lane = threadIdx.x & 31;
+  if (n > most && bound) {
+    int c = 0;
+    for (int i = lane; i < n_mine; i += 32) c += mine[i] >= bound;
+    c = __reduce_add_sync(0xFFFFFFFFu, c);
+    if (lane == 0) atomicAdd(&sh.n_last, c);
+    __syncthreads();
+    n = sh.n_last;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n_last = 0;
+    __syncthreads();
+  }
+  if (n > most) bound = select_bound<kThr>(mine, n_mine, k, bits, sh);
+  for (int i = lane; i < n_mine; i += 32)
+    if (mine[i] >= bound) sh.last[atomicAdd(&sh.n_last, 1)] = mine[i];
   __syncthreads();
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
-  for (int i = threadIdx.x & 31; i < n_mine; i += 32)
-    if (mine[i] >= bound) out[atomicAdd(&sh.n, 1)] = mine[i];
-  __syncthreads();
-  return n > most ? k : n;
+  return sh.n_last;
 }
 
 // One CTA per row, or a cluster of 2 to 8 that share a row's units and bring their parts to the first of them.
-template <class T, int kThr, int kMode>
-__global__ void __launch_bounds__(kThr, (kMode == kTopK ? 4 : 6) * 256 / kThr) rowstat_kernel(const StatArgs a) {
+// kAhead: tiles whose loads are in flight together, 2 where few CTAs run.
+template <class T, int kThr, int kMode, int kAhead>
+__global__ void __launch_bounds__(kThr, (kAhead > 1 ? 2 : kMode == kTopK ? 4 : 6) * 256 / kThr)
+    rowstat_kernel(const StatArgs a) {
   constexpr bool kEnt = kMode == kEntropy || kMode == kTopK;
   constexpr bool kTop = kMode == kTopK;
   constexpr int kNWarps = kThr / 32;
@@ -788,24 +835,33 @@ __global__ void __launch_bounds__(kThr, (kMode == kTopK ? 4 : 6) * 256 / kThr) r
   int slot = 0, in_slot = 0;
   uint32_t best[2] = {0, 0}, order = 0;
 
-  for (int u0 = u_begin; u0 < u_end; u0 += kTile) {
-    Unit<T> w[T::kUnits];
-    load_tile<T, kThr>(x, u0, u_end, w);
-    float cm = unit_max<T>(w[0]);
+  if (kTop && tid == 0) sh.items = sh.n = sh.n_last = 0;
+
+  for (int first = u_begin; first < u_end; first += kAhead * kTile) {
+    Unit<T> w[kAhead][T::kUnits];
 #pragma unroll
-    for (int u = 1; u < T::kUnits; ++u) cm = maxn(cm, unit_max<T>(w[u]));
-    fold_tile<T, kEnt>(w, cm, st, c2);
-    if constexpr (kTop) {
-      order = max(order, order16<T>(cm));
-      if (++in_slot == per_slot || u0 + kTile >= u_end) {
-        table[slot * kThr + tid] = static_cast<uint16_t>(order);
-        if (slot & 1)
-          best[1] = max(best[1], order);
-        else
-          best[0] = max(best[0], order);
-        ++slot;
-        in_slot = 0;
-        order = 0;
+    for (int h = 0; h < kAhead; ++h)
+      if (h == 0 || first + h * kTile < u_end) load_tile<T, kThr>(x, first + h * kTile, u_end, w[h]);
+#pragma unroll
+    for (int h = 0; h < kAhead; ++h) {
+      const int u0 = first + h * kTile;
+      if (h > 0 && u0 >= u_end) break;
+      float cm = unit_max<T>(w[h][0]);
+#pragma unroll
+      for (int u = 1; u < T::kUnits; ++u) cm = maxn(cm, unit_max<T>(w[h][u]));
+      fold_tile<T, kEnt>(w[h], cm, st, c2);
+      if constexpr (kTop) {
+        order = max(order, order16<T>(cm));
+        if (++in_slot == per_slot || u0 + kTile >= u_end) {
+          table[slot * kThr + tid] = static_cast<uint16_t>(order);
+          if (slot & 1)
+            best[1] = max(best[1], order);
+          else
+            best[0] = max(best[0], order);
+          ++slot;
+          in_slot = 0;
+          order = 0;
+        }
       }
     }
   }
@@ -817,20 +873,18 @@ __global__ void __launch_bounds__(kThr, (kMode == kTopK ? 4 : 6) * 256 / kThr) r
   if (warp == 0) {
     st = tid < kNWarps ? sh_stat[tid] : Stat{kNegInf, 0.0f, 0.0f};
     st = warp_merge(st, c2);
-    if constexpr (kTop) {
-      const uint32_t r = reached_by<kThr>(sh.maxima, a.k);
-      if (tid == 0) {
-        sh.reached = r;
-        sh.items = sh.n = 0;
-      }
-    }
   }
   const uint64_t* mine = nullptr;
   int n_mine = 0, n = 0;
   const int bits = T::kKeyBits + a.ib;
+  uint64_t bound = 0;
   if constexpr (kTop) {
+    if (warp == 1) {
+      const uint32_t r = reached_by<kThr>(sh.maxima, a.k);
+      if ((tid & 31) == 0) sh.reached = r;
+    }
     __syncthreads();
-    n = find_top<T, kThr>(x, u_begin, u_end, per_slot, slot, a.k, a.ib, mem, sh, &mine, &n_mine);
+    n = find_top<T, kThr>(x, u_begin, u_end, per_slot, slot, max(best[0], best[1]), a.k, a.ib, mem, sh, &mine, &n_mine);
   }
 
   if (n_parts > 1) {
@@ -838,10 +892,12 @@ __global__ void __launch_bounds__(kThr, (kMode == kTopK ? 4 : 6) * 256 / kThr) r
     uint64_t* part_keys = reinterpret_cast<uint64_t*>(mem + TopLayout<kThr>::kBytes);  // [n_parts][cap]
     if constexpr (kTop) {
       if (n > a.cap) {
-        n = collect<kThr>(mine, n_mine, n, a.k, a.cap, bits, sh.last, sh);
+        n = collect<kThr>(mine, n_mine, n, a.k, a.k, 0, bits, sh);
         const int per = (n + kNWarps - 1) / kNWarps;
         mine = sh.last + warp * per;
         n_mine = max(0, min(per, n - warp * per));
+        __syncthreads();
+        if (tid == 0) sh.n_last = 0;
       }
       if (tid == 0) sh.n = 0;
       __syncthreads();
@@ -855,6 +911,7 @@ __global__ void __launch_bounds__(kThr, (kMode == kTopK ? 4 : 6) * 256 / kThr) r
       PartsShared* to = cluster.map_shared_rank(&parts, 0);
       to->stat[part] = st;
       to->count[part] = n;
+      if constexpr (kTop) to->reached[part] = sh.reached;
     }
     cluster.sync();
     if (part > 0) return;
@@ -867,7 +924,12 @@ __global__ void __launch_bounds__(kThr, (kMode == kTopK ? 4 : 6) * 256 / kThr) r
       mine = part_keys + warp * a.cap;
       n_mine = warp < n_parts ? parts.count[warp] : 0;
       n = 0;
-      for (int i = 0; i < n_parts; ++i) n += parts.count[i];
+      uint32_t reached = 0;  // k elements of one part reach its bound, so the row's k largest do
+      for (int i = 0; i < n_parts; ++i) {
+        n += parts.count[i];
+        reached = max(reached, parts.reached[i]);
+      }
+      bound = static_cast<uint64_t>(reached) << (bits - 16);
     }
   }
 
@@ -893,17 +955,25 @@ __global__ void __launch_bounds__(kThr, (kMode == kTopK ? 4 : 6) * 256 / kThr) r
     // V >= k: there are k keys at least.  The keys of one CTA that are not many lie one after another.
     const uint64_t* last = mine - warp * ((n + kNWarps - 1) / kNWarps);
     if (n_parts > 1 || n > kFinal) {
-      n = collect<kThr>(mine, n_mine, n, a.k, kFinal, bits, sh.last, sh);
+      n = collect<kThr>(mine, n_mine, n, a.k, kFinal, bound, bits, sh);
       last = sh.last;
     } else {
       __syncthreads();  // sh.m, sh.ls
     }
     const float m = sh.m, ls = sh.ls;
-    for (int i = tid; i < n; i += kThr) {
-      const uint64_t key = last[i];
+    int group = 1;  // threads that share the comparisons of a key
+    while (group < 8 && 2 * group * n <= kThr) group *= 2;
+    for (int i0 = 0; i0 < n; i0 += kThr / group) {
+      const int i = i0 + tid / group;
+      const uint64_t key = i < n ? last[i] : ~0ull;
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += last[j] > key;
-      if (rank < a.k) {
+#pragma unroll 4
+      for (int j = 2 * (tid % group); j < n; j += 2 * group) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(last + j);
+        rank += (two.x > key) + (j + 1 < n && two.y > key);
+      }
+      for (int o = 1; o < group; o <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, o);
+      if (i < n && tid % group == 0 && rank < a.k) {
         const uint32_t col = key_col(key, a.ib);
         const float xv = T::kWords == 1 ? key_value<T>(key, a.ib) : T::to_f(x.p[col]);
         a.top_lp[static_cast<int64_t>(row) * a.k + rank] = __fmaf_rn(__fsub_rn(xv, m), a.r.inv_t, -ls);
@@ -1161,7 +1231,7 @@ int check_out(const ufp8_logit_rows* x, int64_t outer, int64_t inner, const char
   return UFP8_OK;
 }
 
-template <class T, int kThr, int kMode>
+template <class T, int kThr, int kMode, int kAhead>
 int launch_stat(StatArgs& a, int part_bits, cudaStream_t s) {
   a.part_bits = part_bits;
   a.cap = 2 * a.k;
@@ -1181,11 +1251,11 @@ int launch_stat(StatArgs& a, int part_bits, cudaStream_t s) {
   int cur = 0;
   cudaError_t e = cudaGetDevice(&cur);
   if (e == cudaSuccess && kMode == kTopK && smem_dev != cur) {
-    e = cudaFuncSetAttribute(rowstat_kernel<T, kThr, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(rowstat_kernel<T, kThr, kMode, kAhead>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(TopLayout<kThr>::kBytes + sizeof(uint64_t) * 2 * kMaxTop * kMaxParts));
     smem_dev = cur;
   }
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, rowstat_kernel<T, kThr, kMode>, a);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, rowstat_kernel<T, kThr, kMode, kAhead>, a);
   return e == cudaSuccess ? UFP8_OK : cuda_error(e, "row statistics launch");
 }
 
@@ -1199,10 +1269,12 @@ int launch_stat(StatArgs& a, cudaStream_t s) {
   while (bits < 3 && (a.r.rows << (bits + 1)) <= most && (static_cast<int64_t>(a.r.V) >> bits) > kTile) ++bits;
   // Many short rows: smaller CTAs, more of which are resident, hide each other's ends.
   if (a.r.rows >= 592) {
-    if (a.r.V <= 8192 && a.k <= 64) return launch_stat<T, 64, kMode>(a, 0, s);
-    if (a.r.V <= (kMode == kTopK ? 32768 : 16384) && a.k <= 128) return launch_stat<T, 128, kMode>(a, 0, s);
+    if (a.r.V <= 8192 && a.k <= 64) return launch_stat<T, 64, kMode, 1>(a, 0, s);
+    if (a.r.V <= (kMode == kTopK ? 32768 : 16384) && a.k <= 128) return launch_stat<T, 128, kMode, 1>(a, 0, s);
   }
-  return launch_stat<T, 256, kMode>(a, bits, s);
+  // Two tiles of loads in flight take twice the registers: where two CTAs per SM are all there are.
+  return (a.r.rows << bits) <= 296 ? launch_stat<T, 256, kMode, 2>(a, bits, s)
+                                   : launch_stat<T, 256, kMode, 1>(a, bits, s);
 }
 
 template <int kMode>
