@@ -771,9 +771,13 @@ __device__ __forceinline__ int collect(const uint64_t* mine, int n_mine, int n, 
 }
 
 // One CTA per row, or a cluster of 2 to 8 that share a row's units and bring their parts to the first of them.
-// kAhead: tiles whose loads are in flight together, 2 where few CTAs run.
+// kAhead: tiles whose loads are in flight together, 2 where few CTAs run.  Resident CTAs, measured at 4096 x 128256
+// (2048 x 50257 in f32): without alternatives 6 per SM; with 64 of them 5 (bf16; 4: 227 us, 5: 216 us) or 4 (f32).
+constexpr int min_ctas(bool top, bool f32, int threads, int ahead) {
+  return (ahead > 1 ? 2 : !top ? 6 : f32 || threads < 256 ? 4 : 5) * 256 / threads;
+}
 template <class T, int kThr, int kMode, int kAhead>
-__global__ void __launch_bounds__(kThr, (kAhead > 1 ? 2 : kMode == kTopK ? 4 : 6) * 256 / kThr)
+__global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kWords > 1, kThr, kAhead))
     rowstat_kernel(const StatArgs a) {
   constexpr bool kEnt = kMode == kEntropy || kMode == kTopK;
   constexpr bool kTop = kMode == kTopK;
