@@ -53,42 +53,36 @@ __device__ __forceinline__ uint4 ld16(const void* p) {
 // ---- element types ---------------------------------------------------------------------------
 struct Bf16 {
   using raw = uint16_t;
-  static constexpr int kWords = 1;    // 16-byte words of a unit
-  static constexpr int kUnits = 4;    // units per thread and tile
+  static constexpr int kElems = 8;    // elements of a unit (16 bytes)
   static constexpr int kKeyBits = 16;
   static __device__ __forceinline__ float to_f(raw r) { return __uint_as_float(static_cast<uint32_t>(r) << 16); }
   static __device__ __forceinline__ raw from_f(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 };
 struct F32 {
   using raw = float;
-  static constexpr int kWords = 2;
-  static constexpr int kUnits = 2;
+  static constexpr int kElems = 4;
   static constexpr int kKeyBits = 32;
   static __device__ __forceinline__ float to_f(raw r) { return r; }
   static __device__ __forceinline__ raw from_f(float f) { return f; }
 };
 
+constexpr int kUnits = 4;  // units per thread and tile, per lane and chunk: 64 bytes of loads in flight
+
 template <class T>
 struct Unit {
-  uint4 w[T::kWords];
+  uint4 w;
 };
 
 template <class T>
-__device__ __forceinline__ void unpack(const Unit<T>& u, float (&v)[8]) {
-  if constexpr (T::kWords == 1) {
-    const uint32_t w[4] = {u.w[0].x, u.w[0].y, u.w[0].z, u.w[0].w};
+__device__ __forceinline__ void unpack(const Unit<T>& u, float (&v)[T::kElems]) {
+  const uint32_t w[4] = {u.w.x, u.w.y, u.w.z, u.w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T::kElems == 8) {
       v[2 * i] = __uint_as_float(w[i] << 16);
       v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      v[4 * i] = __uint_as_float(u.w[i].x);
-      v[4 * i + 1] = __uint_as_float(u.w[i].y);
-      v[4 * i + 2] = __uint_as_float(u.w[i].z);
-      v[4 * i + 3] = __uint_as_float(u.w[i].w);
+    } else {
+      v[i] = __uint_as_float(w[i]);
     }
   }
 }
@@ -96,19 +90,14 @@ __device__ __forceinline__ void unpack(const Unit<T>& u, float (&v)[8]) {
 // Element j of a unit, j not known at compile time.
 template <class T>
 __device__ __forceinline__ float pick(const Unit<T>& u, int j) {
-  if constexpr (T::kWords == 1) {
-    const uint32_t lo = (j & 2) ? u.w[0].y : u.w[0].x, hi = (j & 2) ? u.w[0].w : u.w[0].z;
-    const uint32_t w = (j & 4) ? hi : lo;
-    return __uint_as_float((j & 1) ? w & 0xFFFF0000u : w << 16);
-  } else {
-    const uint4 w = (j & 4) ? u.w[1] : u.w[0];
-    const uint32_t a = (j & 1) ? w.y : w.x, b = (j & 1) ? w.w : w.z;
-    return __uint_as_float((j & 2) ? b : a);
-  }
+  constexpr int kPer = T::kElems / 4;  // elements of a 32-bit word
+  const uint32_t lo = (j / kPer & 1) ? u.w.y : u.w.x, hi = (j / kPer & 1) ? u.w.w : u.w.z;
+  const uint32_t w = (j / kPer & 2) ? hi : lo;
+  return __uint_as_float(kPer == 1 ? w : (j & 1) ? w & 0xFFFF0000u : w << 16);
 }
 
-// A row as units of 8 elements that start on 16-byte boundaries: unit i covers the columns
-// [8 i - off, 8 i - off + 8) where off elements lie between the boundary at or below the row's first
+// A row as units of kElems elements that start on 16-byte boundaries: unit i covers the columns from
+// kElems i - off on, where off elements lie between the boundary at or below the row's first
 // element and that element.  Only the first and the last unit can reach outside the row; those read
 // their columns one by one and hold -inf elsewhere.
 template <class T>
@@ -121,29 +110,26 @@ struct Row {
     p = static_cast<const typename T::raw*>(base) + elem;
     off = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(typename T::raw));
     V = v;
-    units = (v + off + 7) >> 3;
+    units = (v + off + T::kElems - 1) / T::kElems;
   }
   // V < 2^31 - 2^20: a column a tile past the row's end still fits
-  __device__ __forceinline__ int col(int i) const { return i * 8 - off; }
+  __device__ __forceinline__ int col(int i) const { return i * T::kElems - off; }
   __device__ __forceinline__ Unit<T> load(int i) const {
     const int c = col(i);
     Unit<T> u;
-    if (c >= 0 && c + 8 <= V) {
-#pragma unroll
-      for (int k = 0; k < T::kWords; ++k) u.w[k] = ld16(reinterpret_cast<const uint4*>(p + c) + k);
+    if (c >= 0 && c + T::kElems <= V) {
+      u.w = ld16(p + c);
     } else {
-      float v[8];
+      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (c + j >= 0 && c + j < V) ? T::to_f(p[c + j]) : kNegInf;
-      uint32_t* w = &u.w[0].x;
-      if constexpr (T::kWords == 1) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = (__float_as_uint(v[2 * j]) >> 16) | (__float_as_uint(v[2 * j + 1]) & 0xFFFF0000u);
-      } else {
-        u.w[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-        u.w[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+      for (int j = 0; j < T::kElems; ++j) {
+        const uint32_t b = __float_as_uint((c + j >= 0 && c + j < V) ? T::to_f(p[c + j]) : kNegInf);
+        if constexpr (T::kElems == 8)
+          w[j / 2] = j % 2 ? (w[j / 2] | (b & 0xFFFF0000u)) : b >> 16;
+        else
+          w[j] = b;
       }
+      u.w = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return u;
   }
@@ -244,32 +230,32 @@ __device__ __forceinline__ Stat warp_merge(Stat a, float c2) {
 // The maximum of a unit, NaN if one of its elements is.
 template <class T>
 __device__ __forceinline__ float unit_max(const Unit<T>& u) {
-  if constexpr (T::kWords == 1) {
+  if constexpr (T::kElems == 8) {
     uint32_t a, b;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(u.w[0].x), "r"(u.w[0].y));
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(u.w[0].z), "r"(u.w[0].w));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(u.w.x), "r"(u.w.y));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(u.w.z), "r"(u.w.w));
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
     return maxn(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
   } else {
-    float v[8];
+    float v[4];
     unpack<T>(u, v);
-    return maxn(maxn(maxn(v[0], v[1]), maxn(v[2], v[3])), maxn(maxn(v[4], v[5]), maxn(v[6], v[7])));
+    return maxn(maxn(v[0], v[1]), maxn(v[2], v[3]));
   }
 }
 
 // A thread's units of one tile into its running statistics; cm is their maximum.
 template <class T, bool kEnt>
-__device__ __forceinline__ void fold_tile(const Unit<T> (&w)[T::kUnits], float cm, Stat& a, float c2) {
+__device__ __forceinline__ void fold_tile(const Unit<T> (&w)[kUnits], float cm, Stat& a, float c2) {
   if (!(cm <= a.m)) rescale(a, cm, c2);
   const float mz = a.m == kNegInf ? 0.0f : a.m;
   const uint64_t nm = pk(-mz, -mz), c22 = pk(c2, c2);
   uint64_t s = 0, t = 0;
 #pragma unroll
-  for (int u = 0; u < T::kUnits; ++u) {
-    float v[8];
+  for (int u = 0; u < kUnits; ++u) {
+    float v[T::kElems];
     unpack<T>(w[u], v);
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
+    for (int j = 0; j < T::kElems; j += 2) {
       float z0, z1;
       uint64_t z = mul2(add2(pk(v[j], v[j + 1]), nm), c22);
       unpk(z, z0, z1);
@@ -324,7 +310,7 @@ __device__ __forceinline__ uint32_t order16(float x) {
   return static_cast<uint32_t>(make_key<T>(x, 0, 1) >> (T::kKeyBits - 16 + 1));
 }
 
-constexpr int kRegion = 512;  // candidate keys of a warp; at least kMaxTop + the 256 columns of a unit
+constexpr int kRegion = 512;  // candidate keys of a warp; at least kMaxTop + the 256 columns of a warp's units
 constexpr int kSlots = 32;    // entries per thread of the table of maxima
 constexpr int kFinal = 256;   // keys that are put in order by comparing all with all; >= kMaxTop
 constexpr int kMaxParts = 8;  // CTAs of a cluster that share a row
@@ -486,16 +472,17 @@ __device__ uint64_t select_bound(const uint64_t* mine, int n_mine, int k, int bi
   return bound;
 }
 
-// Bit j: element j of the unit at columns c ... c + 7 lies in the row and is not <= thr.
+// Bit j: element j of the unit at columns from c on lies in the row and is not <= thr.
 template <class T>
 __device__ __forceinline__ unsigned above(const Unit<T>& w, float thr, int c, int V) {
-  float v[8];
+  constexpr int kE = T::kElems;
+  float v[kE];
   unpack<T>(w, v);
   unsigned hit = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) hit |= !(v[j] <= thr) ? 1u << j : 0u;
-  if (c < 0) hit &= 0xFFu << min(-c, 8);
-  if (c + 8 > V) hit &= 0xFFu >> min(c + 8 - V, 8);
+  for (int j = 0; j < kE; ++j) hit |= !(v[j] <= thr) ? 1u << j : 0u;
+  if (c < 0) hit &= 0xFFu << min(-c, kE);
+  if (c + kE > V) hit &= ((1u << kE) - 1u) >> min(c + kE - V, kE);
   return hit;
 }
 
@@ -511,7 +498,7 @@ struct Search {
   float thr;
   __device__ __forceinline__ Search(uint64_t* region, int k_, int ib_, uint32_t reached)
       : keys(region), k(k_), ib(ib_), thr(below_order(reached)) {}
-  // unit: 8 columns from c on for every lane, right of all columns before
+  // unit: the columns from c on for every lane, right of all columns before
   __device__ __forceinline__ void take(const Unit<T>& unit, float mx, int c, int V) {
     unsigned hit = !(mx <= thr) ? above<T>(unit, thr, c, V) : 0;
     unsigned who = __ballot_sync(0xFFFFFFFFu, hit != 0);
@@ -621,24 +608,22 @@ __device__ __forceinline__ float distill_row(const StatArgs& a, int64_t base, co
 enum Mode { kPlain = 0, kEntropy = 1, kTopK = 2, kTeacher = 3 };  // kTopK: with the entropy
 
 template <class T, int kThr>
-__device__ __forceinline__ void load_tile(const Row<T>& x, int u0, int u_end, Unit<T> (&w)[T::kUnits]) {
+__device__ __forceinline__ void load_tile(const Row<T>& x, int u0, int u_end, Unit<T> (&w)[kUnits]) {
   const int tid = threadIdx.x;
-  constexpr int kTile = kThr * T::kUnits;
+  constexpr int kTile = kThr * kUnits;
   if (u0 + kTile <= u_end && x.col(u0) >= 0 && x.col(u0 + kTile) <= x.V) {
-    const uint4* p = reinterpret_cast<const uint4*>(x.p + x.col(u0)) + tid * T::kWords;
+    const uint4* p = reinterpret_cast<const uint4*>(x.p + x.col(u0)) + tid;
 #pragma unroll
-    for (int u = 0; u < T::kUnits; ++u)
-#pragma unroll
-      for (int k = 0; k < T::kWords; ++k) w[u].w[k] = ld16(p + u * kThr * T::kWords + k);
+    for (int u = 0; u < kUnits; ++u) w[u].w = ld16(p + u * kThr);
   } else {
-    constexpr uint32_t kFill = T::kWords == 1 ? 0xFF80FF80u : 0xFF800000u;  // -inf
+    constexpr uint32_t kFill = T::kElems == 8 ? 0xFF80FF80u : 0xFF800000u;  // -inf
 #pragma unroll
-    for (int u = 0; u < T::kUnits; ++u) {
+    for (int u = 0; u < kUnits; ++u) {
       const int i = u0 + u * kThr + tid;
       if (i < u_end)
         w[u] = x.load(i);
       else
-        w[u].w[0] = w[u].w[T::kWords - 1] = make_uint4(kFill, kFill, kFill, kFill);
+        w[u].w = make_uint4(kFill, kFill, kFill, kFill);
     }
   }
 }
@@ -648,11 +633,11 @@ template <class T, int kThr>
 __device__ __noinline__ int search_row(const Row<T>& x, int u_begin, int u_end, int k, int ib, uint32_t reached,
                                        uint64_t* region) {
   Search<T> top(region, k, ib, reached);
-  for (int u0 = u_begin; u0 < u_end; u0 += kThr * T::kUnits) {
-    Unit<T> w[T::kUnits];
+  for (int u0 = u_begin; u0 < u_end; u0 += kThr * kUnits) {
+    Unit<T> w[kUnits];
     load_tile<T, kThr>(x, u0, u_end, w);
 #pragma unroll
-    for (int u = 0; u < T::kUnits; ++u)
+    for (int u = 0; u < kUnits; ++u)
       top.take(w[u], unit_max<T>(w[u]), x.col(u0 + u * kThr + threadIdx.x), x.V);
   }
   return top.n;
@@ -668,7 +653,7 @@ __device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end,
                                         int k, int ib, char* mem, TopShared<kThr>& sh, const uint64_t** mine,
                                         int* n_mine) {
   using L = TopLayout<kThr>;
-  constexpr int kTile = kThr * T::kUnits;
+  constexpr int kTile = kThr * kUnits;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint16_t* table = reinterpret_cast<const uint16_t*>(mem);
   uint32_t* items = reinterpret_cast<uint32_t*>(mem + L::kTableBytes);
@@ -698,7 +683,7 @@ __device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end,
   if (m <= L::kItems) {
     constexpr int kFlight = 2;  // units per thread whose loads are in flight together
 #pragma unroll 1
-    for (int q0 = tid; q0 < m * T::kUnits; q0 += kFlight * kThr) {
+    for (int q0 = tid; q0 < m * kUnits; q0 += kFlight * kThr) {
 #pragma unroll 1
       for (int tile = 0; tile < per_slot; ++tile) {
         Unit<T> w[kFlight];
@@ -707,9 +692,9 @@ __device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end,
         for (int f = 0; f < kFlight; ++f) {
           const int q = q0 + f * kThr;
           i[f] = u_end;
-          if (q < m * T::kUnits) {
-            const uint32_t item = items[q / T::kUnits];
-            i[f] = u_begin + (static_cast<int>(item >> 16) * per_slot + tile) * kTile + q % T::kUnits * kThr +
+          if (q < m * kUnits) {
+            const uint32_t item = items[q / kUnits];
+            i[f] = u_begin + (static_cast<int>(item >> 16) * per_slot + tile) * kTile + q % kUnits * kThr +
                    (item & 0xFFFFu);
             if (i[f] < u_end) w[f] = x.load(i[f]);
           }
@@ -777,12 +762,12 @@ constexpr int min_ctas(bool top, bool f32, int threads, int ahead) {
   return (ahead > 1 ? 2 : !top ? 6 : f32 || threads < 256 ? 4 : 5) * 256 / threads;
 }
 template <class T, int kThr, int kMode, int kAhead>
-__global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kWords > 1, kThr, kAhead))
+__global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kKeyBits > 16, kThr, kAhead))
     rowstat_kernel(const StatArgs a) {
   constexpr bool kEnt = kMode == kEntropy || kMode == kTopK;
   constexpr bool kTop = kMode == kTopK;
   constexpr int kNWarps = kThr / 32;
-  constexpr int kTile = kThr * T::kUnits;  // units of a tile
+  constexpr int kTile = kThr * kUnits;  // units of a tile
   extern __shared__ __align__(16) char mem[];  // kTop: TopLayout, then the keys of the cluster's CTAs
   __shared__ Stat sh_stat[kNWarps];
   __shared__ PartsShared parts;
@@ -811,7 +796,7 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kWords > 1, 
   if (n_parts > 1) cg::this_cluster().barrier_arrive();  // "started", awaited before the others' memory is used
 
   const Row<T> x(a.r.x, RowIndex(a.r, row).elem(a.r.stride_outer, a.r.stride_inner), a.r.V);
-  // This CTA's units; parts begin at a multiple of 8 units (128 bytes of bf16).
+  // This CTA's units; parts begin at a multiple of 8 units (128 bytes).
   const int per_part = n_parts == 1 ? x.units : (((x.units + n_parts - 1) >> a.part_bits) + 7) & ~7;
   const int u_begin = min(part * per_part, x.units), u_end = min(u_begin + per_part, x.units);
 
@@ -842,7 +827,7 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kWords > 1, 
   if (kTop && tid == 0) sh.items = sh.n = sh.n_last = 0;
 
   for (int first = u_begin; first < u_end; first += kAhead * kTile) {
-    Unit<T> w[kAhead][T::kUnits];
+    Unit<T> w[kAhead][kUnits];
 #pragma unroll
     for (int h = 0; h < kAhead; ++h)
       if (h == 0 || first + h * kTile < u_end) load_tile<T, kThr>(x, first + h * kTile, u_end, w[h]);
@@ -852,7 +837,7 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kWords > 1, 
       if (h > 0 && u0 >= u_end) break;
       float cm = unit_max<T>(w[h][0]);
 #pragma unroll
-      for (int u = 1; u < T::kUnits; ++u) cm = maxn(cm, unit_max<T>(w[h][u]));
+      for (int u = 1; u < kUnits; ++u) cm = maxn(cm, unit_max<T>(w[h][u]));
       fold_tile<T, kEnt>(w[h], cm, st, c2);
       if constexpr (kTop) {
         order = max(order, order16<T>(cm));
@@ -979,7 +964,7 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kWords > 1, 
       for (int o = 1; o < group; o <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, o);
       if (i < n && tid % group == 0 && rank < a.k) {
         const uint32_t col = key_col(key, a.ib);
-        const float xv = T::kWords == 1 ? key_value<T>(key, a.ib) : T::to_f(x.p[col]);
+        const float xv = T::kKeyBits == 16 ? key_value<T>(key, a.ib) : T::to_f(x.p[col]);
         a.top_lp[static_cast<int64_t>(row) * a.k + rank] = __fmaf_rn(__fsub_rn(xv, m), a.r.inv_t, -ls);
         a.top_id[static_cast<int64_t>(row) * a.k + rank] = col;
       }
@@ -1041,10 +1026,11 @@ __device__ __forceinline__ void load_entry(const GradArgs& a, int64_t row, int j
 // v = p * factor + weight, and a lane with a weight in its columns sets those back to zero.
 template <class T, bool kDistill>
 __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) {
-  constexpr int kChunk = 32 * T::kUnits;  // units of a chunk
-  extern __shared__ float4 wt_all[];      // kWarps * kChunk * 8 floats
+  constexpr int kChunk = 32 * kUnits;  // units of a chunk
+  constexpr int kE = T::kElems;
+  extern __shared__ float4 wt_all[];    // kWarps * kChunk * kE floats
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float4* wt4 = wt_all + warp * kChunk * 2;
+  float4* wt4 = wt_all + warp * kChunk * (kE / 4);
   float* wt = reinterpret_cast<float*>(wt4);
   // unit wi = (row, task) = (wi / tasks, wi % tasks), advanced by the grid's warps without divisions
   const int rows = static_cast<int>(a.r.rows);
@@ -1054,7 +1040,7 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
   const uint64_t c22 = pk(a.r.c2, a.r.c2);
   const int n = kDistill ? a.K : (a.dlogprob ? 1 : 0) + (a.dtop ? a.k : 0);
   if (n > 0)
-    for (int i = lane; i < kChunk * 2; i += 32) wt4[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = lane; i < kChunk * (kE / 4); i += 32) wt4[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   __syncwarp();
   for (; row < rows; row += step_r, task += step_t) {
     if (task >= a.tasks) {
@@ -1094,18 +1080,16 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
     for (; u0 < u_end; u0 += kChunk) {
       const int lo = x.col(u0), hi = x.col(u0 + kChunk);
       const bool whole = lo >= 0 && hi <= x.V && vec;  // every unit is 16-byte loads and stores
-      Unit<T> w[T::kUnits];
+      Unit<T> w[kUnits];
       unsigned flag = 0;  // bit u: unit u of this lane holds a weight
       if (!dead) {
         if (whole) {
-          const uint4* p = reinterpret_cast<const uint4*>(x.p + lo) + lane * T::kWords;
+          const uint4* p = reinterpret_cast<const uint4*>(x.p + lo) + lane;
 #pragma unroll
-          for (int u = 0; u < T::kUnits; ++u)
-#pragma unroll
-            for (int k = 0; k < T::kWords; ++k) w[u].w[k] = ld16(p + u * 32 * T::kWords + k);
+          for (int u = 0; u < kUnits; ++u) w[u].w = ld16(p + u * 32);
         } else {
 #pragma unroll
-          for (int u = 0; u < T::kUnits; ++u) {
+          for (int u = 0; u < kUnits; ++u) {
             const int i = u0 + u * 32 + lane;
             if (i < x.units) w[u] = x.load(i);
           }
@@ -1127,32 +1111,37 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
             const int src = __ffs(left) - 1;
             const int sat = __shfl_sync(0xFFFFFFFFu, at, src);
             const float sw = __shfl_sync(0xFFFFFFFFu, ew, src);
-            if (lane == ((sat >> 3) & 31)) {  // the lane that owns the column
+            if (lane == (sat / kE & 31)) {  // the lane that owns the column
               wt[sat] = __fadd_rn(wt[sat], sw);
-              flag |= 1u << (sat >> 8);
+              flag |= 1u << (sat / (32 * kE));
             }
           }
         }
       }
 #pragma unroll
-      for (int u = 0; u < T::kUnits; ++u) {
+      for (int u = 0; u < kUnits; ++u) {
         const int i = u0 + u * 32 + lane;
         if (!whole && i >= x.units) continue;
-        float v[8];
+        float v[kE];
         if (dead) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+          for (int j = 0; j < kE; ++j) v[j] = 0.0f;
         } else {
           unpack<T>(w[u], v);
-          float e[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+          float e[kE];
+#pragma unroll
+          for (int j = 0; j < kE; ++j) e[j] = 0.0f;
           if ((flag >> u) & 1u) {
-            float4* q = wt4 + (u * 32 + lane) * 2;
-            const float4 q0 = q[0], q1 = q[1];
-            e[0] = q0.x, e[1] = q0.y, e[2] = q0.z, e[3] = q0.w, e[4] = q1.x, e[5] = q1.y, e[6] = q1.z, e[7] = q1.w;
-            q[0] = q[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4* q = wt4 + (u * 32 + lane) * (kE / 4);
+#pragma unroll
+            for (int j = 0; j < kE; j += 4) {
+              const float4 f = q[j / 4];
+              e[j] = f.x, e[j + 1] = f.y, e[j + 2] = f.z, e[j + 3] = f.w;
+              q[j / 4] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
           }
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
+          for (int j = 0; j < kE; j += 2) {
             // log2 p; below -160 the power is 0 and 0 * log2 p has to stay 0
             float z0, z1;
             unpk(fma2(add2(pk(v[j], v[j + 1]), nm), c22, nl), z0, z1);
@@ -1165,23 +1154,21 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
           }
         }
         const int c = x.col(i);
-        if (whole || (vec && c >= 0 && c + 8 <= x.V)) {
-          if constexpr (T::kWords == 1) {
-            uint4 q;
-            uint32_t* qw = &q.x;
+        if (whole || (vec && c >= 0 && c + kE <= x.V)) {
+          uint32_t q[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (kE == 8) {
               const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-              qw[j] = *reinterpret_cast<const uint32_t*>(&b);
+              q[j] = *reinterpret_cast<const uint32_t*>(&b);
+            } else {
+              q[j] = __float_as_uint(v[j]);
             }
-            *reinterpret_cast<uint4*>(o + c) = q;
-          } else {
-            reinterpret_cast<float4*>(o + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(o + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
           }
+          *reinterpret_cast<uint4*>(o + c) = make_uint4(q[0], q[1], q[2], q[3]);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < kE; ++j)
             if (c + j >= 0 && c + j < x.V) o[c + j] = T::from_f(v[j]);
         }
       }
@@ -1265,7 +1252,7 @@ int launch_stat(StatArgs& a, int part_bits, cudaStream_t s) {
 
 template <class T, int kMode>
 int launch_stat(StatArgs& a, cudaStream_t s) {
-  constexpr int kTile = 256 * T::kUnits * 8;  // columns
+  constexpr int kTile = 256 * kUnits * T::kElems;  // columns
   // Few rows: a row is split as long as its parts are whole tiles and all CTAs run at once (those that
   // search for alternatives take more of an SM).
   const int64_t most = kMode == kTopK ? 400 : 800;
@@ -1288,11 +1275,11 @@ int launch_stat(StatArgs& a, int dtype, cudaStream_t s) {
 
 template <class T, bool kDistill>
 int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
-  constexpr int kChunk = 32 * T::kUnits;
+  constexpr int kChunk = 32 * kUnits;
   // a row that starts off a 16-byte boundary can need one unit more
-  const int64_t chunks = ((static_cast<int64_t>(a.r.V) + 7) / 8 + 1 + kChunk - 1) / kChunk;
+  const int64_t chunks = ((static_cast<int64_t>(a.r.V) + T::kElems - 1) / T::kElems + 1 + kChunk - 1) / kChunk;
   const bool entries = kDistill ? a.K > 0 : (a.dlogprob || a.dtop);
-  const size_t smem = entries ? sizeof(float) * 8 * kChunk * kWarps : 0;
+  const size_t smem = entries ? sizeof(float) * T::kElems * kChunk * kWarps : 0;
   // one wave: CTAs beyond the resident ones would start when the first are done
   static thread_local int dev_of[2] = {-1, -1}, per_sm[2] = {0, 0};
   if (dev_of[entries] != dev.device) {

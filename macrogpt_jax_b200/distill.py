@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import ops
-from .logprobs import check_ids, check_logits, check_mask, check_temperature
+from .logprobs import check_ids, check_logits, check_mask, check_temperature, first_order
 
 MAX_ENTRIES = 1024
 
@@ -28,7 +28,7 @@ class _DistillFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, dloss):
         logits, ids, teacher, mask, stats = ctx.saved_tensors
         dlogits = ops.distill_backward(logits, stats, ids, teacher, mask, ctx.temperature, dloss)

@@ -70,19 +70,29 @@ def check_ids(ids: torch.Tensor, shape, logits: torch.Tensor, name: str, who: st
     return ids.contiguous()
 
 
+def first_order(backward):
+    """once_differentiable, without its host time where no graph of the gradient is asked for."""
+    once = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, mask, top_k, temperature, entropy):
-        out = ops.token_logprobs_forward(logits, tokens, mask, top_k, temperature, entropy, True)
+        lp, ent, top_lp, top_id, stats = ops.token_logprobs_forward(logits, tokens, mask, top_k, temperature, entropy,
+                                                                    True)
         if top_k:
-            ctx.mark_non_differentiable(out[3])
+            ctx.mark_non_differentiable(top_id)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, tokens, mask, out[4], out[3])
+        ctx.save_for_backward(logits, tokens, mask, stats, top_id)
         ctx.temperature = temperature
-        return out[:4]
+        return lp, ent, top_lp, top_id
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, dlp, dent, dtop, _):
         logits, tokens, mask, stats, top_id = ctx.saved_tensors
         if dlp is None and dent is None and dtop is None:

@@ -549,14 +549,18 @@ def _empty_f32(shape, device) -> torch.Tensor:
     return torch.empty(*(shape or ((),)), dtype=torch.float32, device=device)
 
 
-def _launch_on(device: torch.device, kind: str, work: float, fn) -> None:
-    """fn(stream) on the current stream of `device`, which may be another one than the current device."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        _launch(kind, work, lambda: fn(torch.cuda.current_stream(index).cuda_stream))
-    else:
+def _launch_on(t: torch.Tensor, kind: str, passes: float, fn) -> None:
+    """fn(stream) on the current stream of t's device, which may be another one than the current device;
+    `passes` over t's bytes are its work."""
+    index = t.device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            _launch(kind, work, lambda: fn(torch.cuda.current_stream(index).cuda_stream))
+            return _launch_on(t, kind, passes, fn)
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if _timer is None:
+        fn(stream)
+    else:
+        _timer.wrap(kind, passes * t.element_size() * t.numel(), lambda: fn(stream))
 
 
 def logit_rows(logits: torch.Tensor) -> LogitRows:
@@ -609,7 +613,7 @@ def token_logprobs_forward(logits: torch.Tensor, tokens: torch.Tensor | None, ma
     top_id = torch.empty(*lead, top_k, dtype=torch.int64, device=dev) if top_k else None
     top_lp = torch.empty_like(top_id, dtype=f32) if top_k else None
     stats = torch.empty(lr.rows, 4, dtype=f32, device=dev) if want_stats else None
-    _launch_on(dev, "logprob", float(t.element_size()) * t.numel(), lambda stream: C.logprob_forward(
+    _launch_on(t, "logprob", 1.0, lambda stream: C.logprob_forward(
         lr.c(temperature, mask), _ptr(tokens), tokens.element_size() if tokens is not None else 0, top_k, _ptr(lp),
         _ptr(ent), _ptr(top_lp), _ptr(top_id), _ptr(stats), stream))
     return lp, ent, top_lp, top_id, stats
@@ -639,7 +643,7 @@ def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: t
     dtop = None if dtop is None else dtop.to(torch.float32).contiguous()
     top_k = top_id.shape[-1] if dtop is not None else 0
     out, outer, inner = _grad_rows(lr)
-    _launch_on(t.device, "logprob_grad", 2.0 * t.element_size() * t.numel(), lambda stream: C.logprob_backward(
+    _launch_on(t, "logprob_grad", 2.0, lambda stream: C.logprob_backward(
         lr.c(temperature, mask), stats.data_ptr(), _ptr(tokens), tokens.element_size() if tokens is not None else 0,
         _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, out.data_ptr(), outer, inner, stream))
     return out
@@ -652,7 +656,7 @@ def distill_forward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tens
     t = lr.logits
     loss = _empty_f32(logits.shape[:-1], t.device)
     stats = torch.empty(lr.rows, 4, dtype=torch.float32, device=t.device) if want_stats else None
-    _launch_on(t.device, "distill", float(t.element_size()) * t.numel(), lambda stream: C.distill_forward(
+    _launch_on(t, "distill", 1.0, lambda stream: C.distill_forward(
         lr.c(temperature, mask), ids.data_ptr(), ids.element_size(), teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype],
         ids.shape[-1], loss.data_ptr(), _ptr(stats), stream))
     return loss, stats
@@ -665,7 +669,7 @@ def distill_backward(logits: torch.Tensor, stats: torch.Tensor, ids: torch.Tenso
     t = lr.logits
     dloss, stride = _row_grad(dloss)
     out, outer, inner = _grad_rows(lr)
-    _launch_on(t.device, "distill_grad", 2.0 * t.element_size() * t.numel(), lambda stream: C.distill_backward(
+    _launch_on(t, "distill_grad", 2.0, lambda stream: C.distill_backward(
         lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(), ids.element_size(), teacher.data_ptr(),
         _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride, out.data_ptr(), outer, inner, stream))
     return out
