@@ -316,11 +316,14 @@ int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens, int token
  * elements, rows apart) for the upstream gradients dlogprob and dentropy (f32, one per row at the given
  * stride; 0: one value for all rows) and dtop (f32 [rows][top_k], with the forward's top_ids); NULL:
  * none.  dentropy needs a forward with `entropy`.  A masked row's gradient is 0.  Every column of every
- * row is written; fastest where an output row starts as far from a 16-byte boundary as its logit row. */
+ * row is written; fastest where an output row starts as far from a 16-byte boundary as its logit row.
+ * For the logits of an output head (bf16 only): cap > 0 says that the logits are cap * tanh(l / cap) and
+ * asks for the gradient at l (times 1 - (x / cap)^2; UFP8_EPI_XENT's soft cap), and *amax (NULL: not
+ * wanted) becomes the largest |dlogits|, for ufp8_quantize. */
 int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const void* tokens, int token_bytes,
                           const float* dlogprob, int64_t dlogprob_stride, const float* dentropy,
                           int64_t dentropy_stride, const float* dtop, const int64_t* top_ids, int64_t top_k,
-                          void* dlogits, int64_t out_stride_outer, int64_t out_stride_inner,
+                          float cap, void* dlogits, int64_t out_stride_outer, int64_t out_stride_inner, float* amax,
                           ufp8_stream_t stream);
 
 /* Distillation from a teacher's top logits.  Per row, `entries` (0..1024) columns teacher_ids (int32 or
@@ -337,8 +340,8 @@ int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teacher_ids, int 
  * rules above; arguments as in ufp8_logprob_backward.  The teacher gets no gradient. */
 int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stats, const void* teacher_ids, int id_bytes,
                           const void* teacher, int teacher_dtype, int64_t entries, const float* dloss,
-                          int64_t dloss_stride, void* dlogits, int64_t out_stride_outer,
-                          int64_t out_stride_inner, ufp8_stream_t stream);
+                          int64_t dloss_stride, float cap, void* dlogits, int64_t out_stride_outer,
+                          int64_t out_stride_inner, float* amax, ufp8_stream_t stream);
 
 /* ---- Newton-Schulz orthogonalisation (Muon) ------------------------------------------------
  * Replaces orthogonalize (ueaj/opt/multiscale.py:110-141): optax.contrib's

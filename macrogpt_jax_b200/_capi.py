@@ -219,9 +219,9 @@ def load() -> ctypes.CDLL:
     lib.ufp8_xent_backward.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, vp, f32, i32, vp, i64, vp, vp, vp]
     rp = ctypes.POINTER(LogitRows)
     lib.ufp8_logprob_forward.argtypes = [rp, vp, i32, i64, vp, vp, vp, vp, vp, vp]
-    lib.ufp8_logprob_backward.argtypes = [rp, vp, vp, i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, i64, vp]
+    lib.ufp8_logprob_backward.argtypes = [rp, vp, vp, i32, vp, i64, vp, i64, vp, vp, i64, f32, vp, i64, i64, vp, vp]
     lib.ufp8_distill_forward.argtypes = [rp, vp, i32, vp, i32, i64, vp, vp, vp]
-    lib.ufp8_distill_backward.argtypes = [rp, vp, vp, i32, vp, i32, i64, vp, i64, vp, i64, i64, vp]
+    lib.ufp8_distill_backward.argtypes = [rp, vp, vp, i32, vp, i32, i64, vp, i64, f32, vp, i64, i64, vp, vp]
     lib.ufp8_newton_schulz_workspace.argtypes = [i64, i64, i64, ctypes.POINTER(i64)]
     lib.ufp8_newton_schulz.argtypes = [vp, i32, i64, i64, i64, i32, vp, f32, vp, i32, vp, i64, vp]
     lib.ufp8_rope_table.argtypes = [vp, i64, i64, vp, vp, vp, vp]
@@ -334,10 +334,10 @@ def logprob_forward(rows: LogitRows, tokens_ptr, token_bytes, top_k, logprob_ptr
 
 
 def logprob_backward(rows: LogitRows, stats_ptr, tokens_ptr, token_bytes, dlp_ptr, dlp_stride, dent_ptr, dent_stride,
-                     dtop_ptr, top_id_ptr, top_k, out_ptr, out_outer, out_inner, stream) -> None:
+                     dtop_ptr, top_id_ptr, top_k, cap, out_ptr, out_outer, out_inner, amax_ptr, stream) -> None:
     check(load().ufp8_logprob_backward(ctypes.byref(rows), stats_ptr, tokens_ptr, token_bytes, dlp_ptr, dlp_stride,
-                                       dent_ptr, dent_stride, dtop_ptr, top_id_ptr, top_k, out_ptr, out_outer,
-                                       out_inner, stream))
+                                       dent_ptr, dent_stride, dtop_ptr, top_id_ptr, top_k, cap, out_ptr, out_outer,
+                                       out_inner, amax_ptr, stream))
     _count(1 if rows.rows > 0 else 0)
 
 
@@ -350,9 +350,10 @@ def distill_forward(rows: LogitRows, ids_ptr, id_bytes, teacher_ptr, teacher_dty
 
 
 def distill_backward(rows: LogitRows, stats_ptr, ids_ptr, id_bytes, teacher_ptr, teacher_dtype, entries, dloss_ptr,
-                     dloss_stride, out_ptr, out_outer, out_inner, stream) -> None:
+                     dloss_stride, cap, out_ptr, out_outer, out_inner, amax_ptr, stream) -> None:
     check(load().ufp8_distill_backward(ctypes.byref(rows), stats_ptr, ids_ptr, id_bytes, teacher_ptr, teacher_dtype,
-                                       entries, dloss_ptr, dloss_stride, out_ptr, out_outer, out_inner, stream))
+                                       entries, dloss_ptr, dloss_stride, cap, out_ptr, out_outer, out_inner, amax_ptr,
+                                       stream))
     _count(1 if rows.rows > 0 else 0)
 
 

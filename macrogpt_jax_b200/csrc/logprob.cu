@@ -193,6 +193,8 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
+
 // ---- running softmax statistics -----------------------------------------------------------------
 struct Stat {
   float m, s, t;
@@ -994,6 +996,8 @@ struct GradArgs {
   int K;
   const float* dloss;
   int64_t dloss_stride;
+  float inv_cap;  // 1 / cap of logits that are cap * tanh(.), 0: not capped
+  uint32_t* amax;  // largest |output| as f32 bits (null: not wanted)
   void* out;
   int64_t out_outer, out_inner;  // row strides of the output
   int tasks;     // tasks of a row
@@ -1024,7 +1028,8 @@ __device__ __forceinline__ void load_entry(const GradArgs& a, int64_t row, int j
 // factors; per chunk it adds the weights of the row's entries that fall into it into `wt`, one f32 per
 // column and zero elsewhere, in entry order, so that the result does not depend on timing.  Then
 // v = p * factor + weight, and a lane with a weight in its columns sets those back to zero.
-template <class T, bool kDistill>
+// kHead: the logits are an output head's (soft cap, largest absolute value for the fp8 scale).
+template <class T, bool kDistill, bool kHead>
 __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) {
   constexpr int kChunk = 32 * kUnits;  // units of a chunk
   constexpr int kE = T::kElems;
@@ -1037,7 +1042,8 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
   const unsigned first = blockIdx.x * kWarps + warp, step = gridDim.x * kWarps;
   const int step_r = static_cast<int>(step / a.tasks), step_t = static_cast<int>(step % a.tasks);
   int row = static_cast<int>(first / a.tasks), task = static_cast<int>(first % a.tasks);
-  const uint64_t c22 = pk(a.r.c2, a.r.c2);
+  const uint64_t c22 = pk(a.r.c2, a.r.c2), cap2 = pk(a.inv_cap, a.inv_cap);
+  float peak = 0.0f;
   const int n = kDistill ? a.K : (a.dlogprob ? 1 : 0) + (a.dtop ? a.k : 0);
   if (n > 0)
     for (int i = lane; i < kChunk * (kE / 4); i += 32) wt4[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1150,7 +1156,13 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
               z1 = maxn(z1, -160.0f);
             }
             const uint64_t f = kDistill ? A2 : fma2(B2, pk(z0, z1), A2);
-            unpk(fma2(pk(ex2a(z0), ex2a(z1)), f, pk(e[j], e[j + 1])), v[j], v[j + 1]);
+            uint64_t d = fma2(pk(ex2a(z0), ex2a(z1)), f, pk(e[j], e[j + 1]));
+            if (kHead && a.inv_cap > 0.0f) {  // times tanh' = 1 - (x / cap)^2
+              const uint64_t t = mul2(pk(v[j], v[j + 1]), cap2);
+              d = mul2(d, fma2(t, neg2(t), pk(1.0f, 1.0f)));
+            }
+            unpk(d, v[j], v[j + 1]);
+            if (kHead) peak = maxn(peak, maxn(fabsf(v[j]), fabsf(v[j + 1])));
           }
         }
         const int c = x.col(i);
@@ -1173,6 +1185,10 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
         }
       }
     }
+  }
+  if (kHead && a.amax) {  // rounding is monotonic: the largest stored value is the largest one rounded
+    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(T::to_f(T::from_f(peak))) & 0x7FFFFFFFu);
+    if (lane == 0) atomicMax(a.amax, bits);
   }
 }
 
@@ -1273,7 +1289,7 @@ int launch_stat(StatArgs& a, int dtype, cudaStream_t s) {
   return dtype == UFP8_OUT_F32 ? launch_stat<F32, kMode>(a, s) : launch_stat<Bf16, kMode>(a, s);
 }
 
-template <class T, bool kDistill>
+template <class T, bool kDistill, bool kHead>
 int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
   constexpr int kChunk = 32 * kUnits;
   // a row that starts off a 16-byte boundary can need one unit more
@@ -1285,7 +1301,7 @@ int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
   if (dev_of[entries] != dev.device) {
     int n = 0;
     const cudaError_t e =
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rowgrad_kernel<T, kDistill>, kThreads, smem);
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rowgrad_kernel<T, kDistill, kHead>, kThreads, smem);
     if (e != cudaSuccess) return cuda_error(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor(row gradient)");
     per_sm[entries] = n < 1 ? 1 : n;
     dev_of[entries] = dev.device;
@@ -1296,9 +1312,35 @@ int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
   while (a.per_task < 4 && a.per_task < chunks && a.r.rows * chunks >= cap * kWarps * 8 * a.per_task) a.per_task *= 2;
   a.tasks = static_cast<int>((chunks + a.per_task - 1) / a.per_task);
   const int64_t work = (a.r.rows * a.tasks + kWarps - 1) / kWarps;
-  rowgrad_kernel<T, kDistill><<<static_cast<unsigned>(work < cap ? work : cap), kThreads, smem, s>>>(a);
+  rowgrad_kernel<T, kDistill, kHead><<<static_cast<unsigned>(work < cap ? work : cap), kThreads, smem, s>>>(a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? UFP8_OK : cuda_error(e, "row gradient launch");
+}
+
+template <bool kDistill>
+int launch_grad(GradArgs& a, int dtype, const DeviceInfo& dev, cudaStream_t s) {
+  if (a.inv_cap > 0.0f || a.amax) {  // checked: bf16
+    if (a.amax) {
+      const cudaError_t e = cudaMemsetAsync(a.amax, 0, sizeof(float), s);
+      if (e != cudaSuccess) return cuda_error(e, "cudaMemsetAsync(amax)");
+    }
+    if (a.r.rows == 0) return UFP8_OK;
+    return launch_grad<Bf16, kDistill, true>(a, dev, s);
+  }
+  return dtype == UFP8_OUT_F32 ? launch_grad<F32, kDistill, false>(a, dev, s)
+                               : launch_grad<Bf16, kDistill, false>(a, dev, s);
+}
+
+// The output head's part of a backward: soft cap and amax, for bf16 logits.
+int head_args(const ufp8_logit_rows* x, float cap, float* amax, GradArgs* a, const char* who) {
+  if (!(cap >= 0.0f) || std::isinf(cap))
+    return set_error(UFP8_ERR_INVALID, "%s: cap must be 0 or a finite positive value", who);
+  if ((cap > 0.0f || amax) && x->dtype != UFP8_OUT_BF16)
+    return set_error(UFP8_ERR_UNSUPPORTED, "%s: cap and amax need bf16 logits", who);
+  if (!al(amax, 4)) return set_error(UFP8_ERR_ALIGN, "%s: amax not 4-byte aligned", who);
+  a->inv_cap = cap > 0.0f ? 1.0f / cap : 0.0f;
+  a->amax = reinterpret_cast<uint32_t*>(amax);
+  return UFP8_OK;
 }
 
 }  // namespace
@@ -1342,21 +1384,23 @@ extern "C" int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens
 extern "C" int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const void* tokens,
                                      int token_bytes, const float* dlogprob, int64_t dlogprob_stride,
                                      const float* dentropy, int64_t dentropy_stride, const float* dtop,
-                                     const int64_t* top_ids, int64_t top_k, void* dlogits,
-                                     int64_t out_stride_outer, int64_t out_stride_inner, ufp8_stream_t stream) {
+                                     const int64_t* top_ids, int64_t top_k, float cap, void* dlogits,
+                                     int64_t out_stride_outer, int64_t out_stride_inner, float* amax,
+                                     ufp8_stream_t stream) {
   const char* who = "ufp8_logprob_backward";
   GradArgs a{};
   if (int rc = rows_args(x, &a.r, who)) return rc;
   if (top_k < 0 || top_k > kMaxTop) return set_error(UFP8_ERR_INVALID, "%s: top_k must be 0..%d", who, kMaxTop);
   if (int rc = check_out(x, out_stride_outer, out_stride_inner, who)) return rc;
+  if (int rc = head_args(x, cap, amax, &a, who)) return rc;
   if (dlogprob)
     if (int rc = check_ids(tokens, token_bytes, "tokens", who)) return rc;
   if (!al(stats, 16)) return set_error(UFP8_ERR_ALIGN, "%s: stats not 16-byte aligned", who);
   if (!al(dlogits, x->dtype == UFP8_OUT_F32 ? 4 : 2))
     return set_error(UFP8_ERR_ALIGN, "%s: dlogits not aligned to their type", who);
-  if (x->rows == 0) return UFP8_OK;
-  if (!stats || !dlogits) return set_error(UFP8_ERR_INVALID, "%s: null stats or dlogits", who);
-  if (dlogprob && !tokens) return set_error(UFP8_ERR_INVALID, "%s: null tokens", who);
+  if (x->rows == 0 && !amax) return UFP8_OK;
+  if (x->rows > 0 && (!stats || !dlogits)) return set_error(UFP8_ERR_INVALID, "%s: null stats or dlogits", who);
+  if (x->rows > 0 && dlogprob && !tokens) return set_error(UFP8_ERR_INVALID, "%s: null tokens", who);
   if (dtop && (!top_ids || top_k == 0)) return set_error(UFP8_ERR_INVALID, "%s: null top_ids", who);
   DeviceInfo* dev;
   if (int rc = device_info(&dev)) return rc;
@@ -1374,7 +1418,7 @@ extern "C" int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stat
   a.out_outer = out_stride_outer;
   a.out_inner = out_stride_inner;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return x->dtype == UFP8_OUT_F32 ? launch_grad<F32, false>(a, *dev, s) : launch_grad<Bf16, false>(a, *dev, s);
+  return launch_grad<false>(a, x->dtype, *dev, s);
 }
 
 namespace {
@@ -1418,18 +1462,20 @@ extern "C" int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teache
 
 extern "C" int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stats, const void* teacher_ids,
                                      int id_bytes, const void* teacher, int teacher_dtype, int64_t entries,
-                                     const float* dloss, int64_t dloss_stride, void* dlogits,
-                                     int64_t out_stride_outer, int64_t out_stride_inner, ufp8_stream_t stream) {
+                                     const float* dloss, int64_t dloss_stride, float cap, void* dlogits,
+                                     int64_t out_stride_outer, int64_t out_stride_inner, float* amax,
+                                     ufp8_stream_t stream) {
   const char* who = "ufp8_distill_backward";
   GradArgs a{};
   if (int rc = rows_args(x, &a.r, who)) return rc;
   if (int rc = distill_check(x, teacher_ids, id_bytes, teacher, teacher_dtype, entries, who)) return rc;
   if (int rc = check_out(x, out_stride_outer, out_stride_inner, who)) return rc;
+  if (int rc = head_args(x, cap, amax, &a, who)) return rc;
   if (!al(stats, 16)) return set_error(UFP8_ERR_ALIGN, "%s: stats not 16-byte aligned", who);
   if (!al(dlogits, x->dtype == UFP8_OUT_F32 ? 4 : 2))
     return set_error(UFP8_ERR_ALIGN, "%s: dlogits not aligned to their type", who);
-  if (x->rows == 0) return UFP8_OK;
-  if (!stats || !dlogits || !dloss) return set_error(UFP8_ERR_INVALID, "%s: null stats, dloss or dlogits", who);
+  if (x->rows == 0 && !amax) return UFP8_OK;
+  if (x->rows > 0 && (!stats || !dlogits || !dloss)) return set_error(UFP8_ERR_INVALID, "%s: null stats, dloss or dlogits", who);
   DeviceInfo* dev;
   if (int rc = device_info(&dev)) return rc;
   a.stats = reinterpret_cast<const float4*>(stats);
@@ -1444,5 +1490,5 @@ extern "C" int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stat
   a.out_outer = out_stride_outer;
   a.out_inner = out_stride_inner;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return x->dtype == UFP8_OUT_F32 ? launch_grad<F32, true>(a, *dev, s) : launch_grad<Bf16, true>(a, *dev, s);
+  return launch_grad<true>(a, x->dtype, *dev, s);
 }

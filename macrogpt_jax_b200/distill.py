@@ -19,6 +19,22 @@ from .logprobs import check_ids, check_logits, check_mask, check_temperature, fi
 MAX_ENTRIES = 1024
 
 
+def check_teacher(teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, logits: torch.Tensor, who: str):
+    """(ids, teacher values), contiguous, for logits (or activations) of the leading shape."""
+    if teacher_ids.dim() < 1 or teacher_ids.shape[-1] > MAX_ENTRIES:
+        raise ValueError(f"{who}: teacher_ids {tuple(teacher_ids.shape)}: at most {MAX_ENTRIES} entries per row")
+    shape = (*logits.shape[:-1], teacher_ids.shape[-1])
+    ids = check_ids(teacher_ids, shape, logits, "teacher_ids", who)
+    if teacher_logits.shape != shape or teacher_logits.device != logits.device:
+        raise ValueError(f"{who}: teacher_logits {tuple(teacher_logits.shape)} on {teacher_logits.device}, expected "
+                         f"{shape} on {logits.device}")
+    if teacher_logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{who}: expected bfloat16 or float32 teacher_logits, got {teacher_logits.dtype}")
+    if torch.is_grad_enabled() and teacher_logits.requires_grad:
+        raise ValueError(f"{who}: the teacher gets no gradient; detach teacher_logits")
+    return ids, teacher_logits.detach().contiguous()
+
+
 class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, mask, temperature):
@@ -50,18 +66,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     who = "topk_distillation_loss"
     check_logits(logits, who)
     temperature = check_temperature(temperature, who)
-    if teacher_ids.dim() < 1 or teacher_ids.shape[-1] > MAX_ENTRIES:
-        raise ValueError(f"{who}: teacher_ids {tuple(teacher_ids.shape)}: at most {MAX_ENTRIES} entries per row")
-    shape = (*logits.shape[:-1], teacher_ids.shape[-1])
-    ids = check_ids(teacher_ids, shape, logits, "teacher_ids", who)
-    if teacher_logits.shape != shape or teacher_logits.device != logits.device:
-        raise ValueError(f"{who}: teacher_logits {tuple(teacher_logits.shape)} on {teacher_logits.device}, expected "
-                         f"{shape} on {logits.device}")
-    if teacher_logits.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"{who}: expected bfloat16 or float32 teacher_logits, got {teacher_logits.dtype}")
-    if torch.is_grad_enabled() and teacher_logits.requires_grad:
-        raise ValueError(f"{who}: the teacher gets no gradient; detach teacher_logits")
-    teacher = teacher_logits.detach().contiguous()
+    ids, teacher = check_teacher(teacher_ids, teacher_logits, logits, who)
     mask = check_mask(mask, logits, who)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillFn.apply(logits, ids, teacher, mask, temperature)

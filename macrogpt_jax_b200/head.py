@@ -12,16 +12,24 @@ that never hands the logits to the caller:
             GEMMs dX = dL W^T and dW = X^T dL, ufp8_rmsnorm_backward.
 The logits are kept from the forward for the backward (2 bytes per logit in HBM) instead of being
 recomputed, which the reference's rematerialised chunks do (one GEMM of 2 T d V FLOPs fewer).
+
+`token_logprobs` and `distillation_loss` put the operators of logprobs.py and distill.py behind the
+same head (the teacher's targets, the scores of sampled tokens, the student's step): one node of the
+same kind, whose backward quantises the operator's bf16 logit gradient with the amax that the gradient
+kernel kept, and runs the two FP8 GEMMs and the norm's backward.
 """
 from __future__ import annotations
 
-from typing import Callable, Optional
+from typing import Callable, NamedTuple, Optional
 
 import torch
 
 from . import ops
 from .configurator import config
 from .einsum import Einsum, Rngs, zeros_init
+from .distill import check_teacher, topk_distillation_loss
+from .logprobs import (TokenLogprobs, check_ids, check_logits, check_mask, check_score, check_temperature, first_order,
+                       token_logprobs)
 from .rmsnorm import RMSNorm
 
 HEAD_CAP = 15.0  # the constant of ueaj/model/model.py:163
@@ -48,6 +56,77 @@ class _HeadXentFn(torch.autograd.Function):
         dx, ds = ops.rmsnorm_backward(x2d, ctx.scale, ctx.centered, rstd, dxn, need_ds)
         dscale = ds.reshape(ctx.scale.shape).to(torch.bfloat16) if need_ds else None
         return dx, dscale, dw, None, None, None, None, None, None
+
+
+class _HeadRowsFn(torch.autograd.Function):
+    """Head -> operator on its logits.  `op` is a _Score or _Distill: forward(logits, want_stats) ->
+    (outputs, stats), backward(logits, stats, ids, grads, head) with the integer outputs `ids`."""
+
+    @staticmethod
+    def forward(ctx, x2d, scale, w, op, centered, eps, cap, bwd_fmt):
+        logits, (qx, rstd, qw) = ops.head_rows_forward(x2d, scale, centered, eps, w, cap)
+        out, stats = op.forward(logits[:, :w.shape[1]], True)
+        ids = [t for t in out if t is not None and not t.is_floating_point()]
+        ctx.mark_non_differentiable(*ids)
+        ctx.set_materialize_grads(False)
+        # all tensors through autograd, which frees them after the backward and notices a change in place
+        ctx.save_for_backward(x2d, scale, logits, stats, rstd, qx.q, qx.inv_scale, qx.amax, qw.q, qw.inv_scale, qw.amax,
+                              *ids, *op.tensors())
+        ctx.op, ctx.n_ids, ctx.V = op, len(ids), w.shape[1]
+        ctx.centered, ctx.cap, ctx.bwd_fmt = centered, cap, bwd_fmt
+        return out
+
+    @staticmethod
+    @first_order
+    def backward(ctx, *grads):
+        if all(g is None for g in grads):
+            return (None,) * 8
+        x2d, scale, logits, stats, rstd, *rest = ctx.saved_tensors
+        qx, qw, ids = ops.Fp8Tensor(*rest[:3]), ops.Fp8Tensor(*rest[3:6]), rest[6:6 + ctx.n_ids]
+        dxn, dw = ops.head_rows_backward(lambda lg, head: ctx.op.backward(lg, stats, ids, grads, head), logits,
+                                         (qx, rstd, qw), ctx.V, ctx.cap, ctx.needs_input_grad[2], ctx.bwd_fmt)
+        need_ds = scale is not None and ctx.needs_input_grad[1]
+        dx, ds = ops.rmsnorm_backward(x2d, scale, ctx.centered, rstd, dxn, need_ds)
+        dscale = ds.reshape(scale.shape).to(torch.bfloat16) if need_ds else None
+        return dx, dscale, dw, None, None, None, None, None
+
+
+class _Score(NamedTuple):
+    tokens: Optional[torch.Tensor]
+    mask: Optional[torch.Tensor]
+    top_k: int
+    temperature: float
+    entropy: bool
+
+    def tensors(self):
+        return self.tokens, self.mask
+
+    def forward(self, logits, want_stats):
+        *out, stats = ops.token_logprobs_forward(logits, self.tokens, self.mask, self.top_k, self.temperature,
+                                                 self.entropy, want_stats)
+        return tuple(out), stats
+
+    def backward(self, logits, stats, ids, grads, head):
+        dlp, dent, dtop, _ = grads
+        ops.token_logprobs_backward(logits, stats, self.tokens, self.mask, self.temperature, dlp, dent, dtop,
+                                    ids[0] if ids else None, head)
+
+
+class _Distill(NamedTuple):
+    ids: torch.Tensor
+    teacher: torch.Tensor
+    mask: Optional[torch.Tensor]
+    temperature: float
+
+    def tensors(self):
+        return self.ids, self.teacher, self.mask
+
+    def forward(self, logits, want_stats):
+        loss, stats = ops.distill_forward(logits, self.ids, self.teacher, self.mask, self.temperature, want_stats)
+        return (loss,), stats
+
+    def backward(self, logits, stats, ids, grads, head):
+        ops.distill_backward(logits, stats, self.ids, self.teacher, self.mask, self.temperature, grads[0], head)
 
 
 @config
@@ -96,3 +175,52 @@ class OutputHead(torch.nn.Module):
         loss = _HeadXentFn.apply(x2d, self.norm.scale, w, labels, mk, self.norm.recenter, self.norm.eps, cap,
                                  ops.FMT_OF_DTYPE[self.lm_head.bwd_dtype])
         return loss.reshape(lead)
+
+    def _rows(self, activations: torch.Tensor, op):
+        """op's outputs on the logits of the flattened activations, through the fused node."""
+        x2d = activations.to(torch.bfloat16).reshape(-1, self.model_d).contiguous()
+        w = self.lm_head.w if self.lm_head.w.dtype == torch.bfloat16 else self.lm_head.w.to(torch.bfloat16)
+        cap = HEAD_CAP if self.head_cap == "tanh" else 0.0
+        scale = self.norm.scale
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2d, scale, w)):
+            return _HeadRowsFn.apply(x2d, scale, w, op, self.norm.recenter, self.norm.eps, cap,
+                                     ops.FMT_OF_DTYPE[self.lm_head.bwd_dtype])
+        logits, _ = ops.head_rows_forward(x2d, scale, self.norm.recenter, self.norm.eps, w, cap)
+        return op.forward(logits[:, :self.vocab_size], False)[0]
+
+    def token_logprobs(self, activations: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
+                       temperature: float = 1.0, mask: Optional[torch.Tensor] = None,
+                       entropy: bool = True) -> TokenLogprobs:
+        """logprobs.token_logprobs(self.get_logits(activations), ...), through the fused node when
+        fused() holds (then the gradients reach the activations, the norm and the lm_head)."""
+        if not self.fused():
+            return token_logprobs(self.get_logits(activations), tokens, top_k=top_k, temperature=temperature, mask=mask,
+                                  entropy=entropy)
+        who, lead = "OutputHead.token_logprobs", activations.shape[:-1]
+        check_logits(activations, who)
+        temperature = check_score(tokens, top_k, self.vocab_size, temperature, entropy, who)
+        if tokens is not None:
+            tokens = check_ids(tokens, lead, activations, "tokens", who).reshape(-1)
+        mask = check_mask(mask, activations, who)
+        op = _Score(tokens, None if mask is None else mask.reshape(-1), top_k, temperature, entropy)
+        lp, ent, top_lp, top_id = self._rows(activations, op)
+        return TokenLogprobs(None if lp is None else lp.reshape(lead), None if ent is None else ent.reshape(lead),
+                             None if top_lp is None else top_lp.reshape(*lead, top_k),
+                             None if top_id is None else top_id.reshape(*lead, top_k))
+
+    def distillation_loss(self, activations: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                          temperature: float = 1.0, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """distill.topk_distillation_loss(self.get_logits(activations), ...), through the fused node when
+        fused() holds."""
+        if not self.fused():
+            return topk_distillation_loss(self.get_logits(activations), teacher_ids, teacher_logits,
+                                          temperature=temperature, mask=mask)
+        who, lead = "OutputHead.distillation_loss", activations.shape[:-1]
+        check_logits(activations, who)
+        temperature = check_temperature(temperature, who)
+        ids, teacher = check_teacher(teacher_ids, teacher_logits, activations, who)
+        mask = check_mask(mask, activations, who)
+        K = ids.shape[-1]
+        op = _Distill(ids.reshape(-1, K), teacher.reshape(-1, K), None if mask is None else mask.reshape(-1),
+                      temperature)
+        return self._rows(activations, op)[0].reshape(lead)

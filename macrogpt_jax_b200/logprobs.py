@@ -44,6 +44,15 @@ def check_temperature(temperature: float, who: str) -> float:
     return t
 
 
+def check_score(tokens, top_k: int, V: int, temperature: float, entropy: bool, who: str) -> float:
+    """What is asked of token_logprobs over V columns; returns the temperature."""
+    if not 0 <= top_k <= MAX_TOP_K or top_k > V:
+        raise ValueError(f"{who}: top_k must be 0..{min(MAX_TOP_K, V)}, got {top_k}")
+    if tokens is None and not entropy and not top_k:
+        raise ValueError(f"{who}: nothing asked for (no tokens, no entropy, top_k 0)")
+    return check_temperature(temperature, who)
+
+
 def check_mask(mask: Optional[torch.Tensor], logits: torch.Tensor, who: str) -> Optional[torch.Tensor]:
     """The mask as contiguous bytes, one per row: 0 leaves the row out."""
     if mask is None:
@@ -118,11 +127,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     who = "token_logprobs"
     check_logits(logits, who)
     lead, V = logits.shape[:-1], logits.shape[-1]
-    temperature = check_temperature(temperature, who)
-    if not 0 <= top_k <= MAX_TOP_K or top_k > V:
-        raise ValueError(f"{who}: top_k must be 0..{min(MAX_TOP_K, V)}, got {top_k}")
-    if tokens is None and not entropy and not top_k:
-        raise ValueError(f"{who}: nothing asked for (no tokens, no entropy, top_k 0)")
+    temperature = check_score(tokens, top_k, V, temperature, entropy, who)
     if tokens is not None:
         tokens = check_ids(tokens, lead, logits, "tokens", who)
     mask = check_mask(mask, logits, who)

@@ -602,6 +602,14 @@ def _grad_rows(lr: LogitRows):
     return buf.as_strided((n_outer, lr.inner, V), (outer, inner, 1), start).view(t.shape), outer, inner
 
 
+def _grad_target(lr: LogitRows, head: tuple | None):
+    """(cap, dlogits, its row strides, amax) of a backward."""
+    if head is None:
+        return (0.0, *_grad_rows(lr), None)
+    cap, out, amax_t = head
+    return cap, out, 0, out.stride(0), amax_t
+
+
 def token_logprobs_forward(logits: torch.Tensor, tokens: torch.Tensor | None, mask: torch.Tensor | None, top_k: int,
                            temperature: float, entropy: bool, want_stats: bool):
     """(logprob, entropy, top log probabilities, top ids) over the logits' leading shape, then the
@@ -633,19 +641,21 @@ def _row_grad(g: torch.Tensor | None):
 
 def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: torch.Tensor | None,
                             mask: torch.Tensor | None, temperature: float, dlp: torch.Tensor | None,
-                            dent: torch.Tensor | None, dtop: torch.Tensor | None,
-                            top_id: torch.Tensor | None) -> torch.Tensor:
-    """dlogits of token_logprobs_forward (ufp8_logprob_backward)."""
+                            dent: torch.Tensor | None, dtop: torch.Tensor | None, top_id: torch.Tensor | None,
+                            head: tuple | None = None) -> torch.Tensor:
+    """dlogits of token_logprobs_forward (ufp8_logprob_backward).  `head`: (soft cap, dlogits buffer
+    [rows, pitch], amax) of an output head, see head_rows_backward."""
     lr = logit_rows(logits)
     t = lr.logits
     dlp, s_lp = _row_grad(dlp)
     dent, s_ent = _row_grad(dent)
     dtop = None if dtop is None else dtop.to(torch.float32).contiguous()
     top_k = top_id.shape[-1] if dtop is not None else 0
-    out, outer, inner = _grad_rows(lr)
+    cap, out, outer, inner, amax_t = _grad_target(lr, head)
     _launch_on(t, "logprob_grad", 2.0, lambda stream: C.logprob_backward(
         lr.c(temperature, mask), stats.data_ptr(), _ptr(tokens), tokens.element_size() if tokens is not None else 0,
-        _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, out.data_ptr(), outer, inner, stream))
+        _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, cap, out.data_ptr(), outer, inner,
+        _ptr(amax_t), stream))
     return out
 
 
@@ -663,16 +673,50 @@ def distill_forward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tens
 
 
 def distill_backward(logits: torch.Tensor, stats: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
-                     mask: torch.Tensor | None, temperature: float, dloss: torch.Tensor) -> torch.Tensor:
-    """dlogits of distill_forward (ufp8_distill_backward)."""
+                     mask: torch.Tensor | None, temperature: float, dloss: torch.Tensor,
+                     head: tuple | None = None) -> torch.Tensor:
+    """dlogits of distill_forward (ufp8_distill_backward); `head` as in token_logprobs_backward."""
     lr = logit_rows(logits)
     t = lr.logits
     dloss, stride = _row_grad(dloss)
-    out, outer, inner = _grad_rows(lr)
+    cap, out, outer, inner, amax_t = _grad_target(lr, head)
     _launch_on(t, "distill_grad", 2.0, lambda stream: C.distill_backward(
         lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(), ids.element_size(), teacher.data_ptr(),
-        _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride, out.data_ptr(), outer, inner, stream))
+        _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride, cap, out.data_ptr(), outer, inner,
+        _ptr(amax_t), stream))
     return out
+
+
+# The same operators behind the fused output head: final norm -> FP8 lm_head (soft cap in its epilogue) ->
+# logits [T, Vp] -> operator, whose dlogits (bf16, with their amax from the same kernel) are quantised for
+# the two backward GEMMs.
+def head_rows_forward(x2d: torch.Tensor, scale: torch.Tensor | None, centered: bool, eps: float, w: torch.Tensor,
+                      cap: float):
+    """(logits bf16 [T, Vp] of which columns < V count, saved)."""
+    x2d = _check_bf16_cuda(x2d, "x")
+    qx, rstd = rmsnorm_quant(x2d, scale, centered, eps, C.E4M3)
+    qw = quantize_head_weight(w)
+    logits, _ = head_logits(qx, qw, w.shape[1], cap)
+    return logits, (qx, rstd, qw)
+
+
+def head_rows_backward(grad_fn, logits: torch.Tensor, saved, V: int, cap: float, need_dw: bool, fmt: int):
+    """Backward of head_rows_forward up to the norm: (dxn bf16 [T, d], dw bf16 [d, V] or None).
+    grad_fn(logits [T, V], head) writes dlogits as token_logprobs_backward and distill_backward do."""
+    qx, _, qw = saved
+    T, d = qx.q.shape
+    dl = torch.empty_like(logits)
+    amax_t = torch.empty(1, dtype=torch.float32, device=logits.device)
+    grad_fn(logits[:, :V], (cap, dl, amax_t))
+    qd = quantize(dl, fmt, amax_t)
+    Vp = logits.shape[1]
+    dxn = torch.empty((T, d), dtype=torch.bfloat16, device=logits.device)
+    gemm(operand(qd, C.K_MAJOR, Vp), operand(qw, C.K_MAJOR, Vp), T, d, V, dxn, d)
+    dw = None
+    if need_dw:
+        dw = torch.empty((d, V), dtype=torch.bfloat16, device=logits.device)
+        gemm(operand(qx, C.MN_MAJOR, d), operand(qd, C.MN_MAJOR, Vp), d, V, T, dw, V)
+    return dxn, dw
 
 
 # ----------------------------------------------------------------------------- Newton-Schulz

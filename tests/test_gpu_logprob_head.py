@@ -1,0 +1,212 @@
+"""OutputHead.token_logprobs and OutputHead.distillation_loss on a B200: the fused node (RMSNorm -> FP8
+lm_head -> soft cap -> operator) against the definitions in 64 bits on plainly computed logits of the same
+fp8 recipe, and its gradients against a plain computation of the same recipe.
+
+Tolerances.  The node's logits and the plain ones are one bf16 rounding of two f32 sums in different
+orders (and a soft cap of three roundings): at most one bf16 step apart, which is 2^-4 for 8 <= |logit| <
+16.  A log probability moves by at most |dx_t| + sum_v p_v |dx_v|, so by two steps: 2^-3.  Gradients go through fp8 GEMMs: the tolerance of helpers.py against a reference
+that quantises the same way.  The logit gradient is checked before the fp8 cast, on the kernels
+themselves: half a bf16 step and the f32 terms of test_gpu_logprob.py."""
+import pytest
+import torch
+
+from helpers import compare
+
+pytestmark = pytest.mark.gpu
+LOGIT = 2.0 ** -3
+
+
+def make_head(cuda, d, V, cap, seed=0):
+    from macrogpt_jax_b200.einsum import Rngs
+    from macrogpt_jax_b200.head import OutputHead
+    head = OutputHead(d, V, head_cap=cap, rngs=Rngs(seed))
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    with torch.no_grad():
+        head.lm_head.w.copy_(torch.randn((d, V), generator=g, device=cuda) * 3 * d ** -0.5)
+        head.norm.scale.copy_(1 + 0.3 * torch.randn(d, generator=g, device=cuda))
+    x = torch.randn((2, 48, d), generator=g, device=cuda).bfloat16()
+    return head, x, g
+
+
+def fp8(t, dt, fmax):
+    s = fmax / t.abs().max().float().clamp(min=1e-30)
+    return (t.float() * s).to(dt).float() / s
+
+
+def plain_operands(head, xn):
+    return (fp8(xn.detach().bfloat16(), torch.float8_e4m3fn, 448.0),
+            fp8(head.lm_head.w.detach(), torch.float8_e4m3fn, 448.0))
+
+
+def capped(head, qx, qw):
+    logits = (qx @ qw).bfloat16().float()
+    if head.head_cap != "tanh":
+        return logits
+    return (15 * torch.tanh((logits / 15).bfloat16().float()).bfloat16().float()).bfloat16().float()
+
+
+def plain_logits(head, x):
+    x = x.detach().float()
+    xn = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + head.norm.eps) * head.norm.scale.detach().float()
+    return capped(head, *plain_operands(head, xn))
+
+
+def head_reference(head, x, grad_logits):
+    """Gradients of sum(<grad_logits(logits), logits>) with the node's recipe: e4m3 operands, the logit
+    gradient in the lm_head's bwd_dtype, both per tensor, f32 products, the norm by autograd."""
+    x = x.detach().float().requires_grad_(True)
+    scale = head.norm.scale.detach().float().requires_grad_(True)
+    xn = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + head.norm.eps) * scale
+    qx, qw = plain_operands(head, xn)
+    c = capped(head, qx, qw)
+    dl = grad_logits(c)
+    if head.head_cap == "tanh":
+        dl = dl * (1 - (c / 15) ** 2)
+    qd = fp8(dl.bfloat16(), torch.float8_e5m2, 57344.0)
+    dw = qx.reshape(-1, qx.shape[-1]).T @ qd.reshape(-1, qd.shape[-1])
+    dxn = (qd @ qw.T).bfloat16().float()
+    dx, ds = torch.autograd.grad(xn, (x, scale), dxn)
+    return dx, ds, dw
+
+
+@pytest.mark.parametrize("cap,V", [(None, 1000), ("tanh", 1000), ("tanh", 2048)])
+def test_head_scores(cuda, cap, V):
+    head, x, g = make_head(cuda, 256, V, cap)
+    tok = torch.randint(0, V, (2, 48), generator=g, device=cuda)
+    mask = torch.rand((2, 48), generator=g, device=cuda) > 0.3
+    with torch.no_grad():
+        out = head.token_logprobs(x, tok, top_k=5, temperature=0.8, mask=mask)
+        logits = plain_logits(head, x)
+    assert logits.abs().max() < 16
+    logp = torch.log_softmax(logits.double() / 0.8, -1)
+    tol = LOGIT / 0.8
+    ref = torch.where(mask, logp.gather(2, tok[..., None])[..., 0], 0.0)
+    assert (out.logprob.double() - ref).abs().max() <= tol
+    H = torch.where(mask, -(logp.exp() * logp).sum(-1), 0.0)
+    # dH/dx_v = -p_v (log p_v + H): at most max(log V, H) in sum
+    assert (out.entropy.double() - H).abs().max() <= tol * 8
+    assert (out.top_ids[~mask] == -1).all()
+    got = logp.gather(2, out.top_ids.clamp(min=0))
+    best = logp.topk(5, dim=-1).values
+    assert ((got - best).abs()[mask] <= tol).all()
+    assert ((out.top_logprobs.double() - best).abs()[mask] <= tol).all()
+
+
+@pytest.mark.parametrize("cap,V", [(None, 1000), ("tanh", 1000), ("tanh", 2048)])
+def test_head_score_gradients(cuda, cap, V):
+    head, x, g = make_head(cuda, 256, V, cap, 3)
+    tok = torch.randint(0, V, (2, 48), generator=g, device=cuda)
+    mask = torch.rand((2, 48), generator=g, device=cuda) > 0.3
+    adv = torch.randn((2, 48), generator=g, device=cuda)
+    x = x.requires_grad_(True)
+    out = head.token_logprobs(x, tok, top_k=3, mask=mask)
+    dtop = torch.randn(out.top_logprobs.shape, generator=g, device=cuda) * 0.1
+    loss = (out.logprob * adv).sum() + 0.05 * out.entropy.sum() + (out.top_logprobs * dtop)[mask].sum()
+    loss.backward()
+
+    def grad(c):
+        c = c.double().requires_grad_(True)
+        lp = torch.log_softmax(c, -1)
+        val = (lp.gather(2, tok[..., None])[..., 0] * adv - 0.05 * (lp.exp() * lp).sum(-1))[mask].sum()
+        val = val + (lp.gather(2, out.top_ids.clamp(min=0)) * dtop)[mask].sum()
+        return torch.autograd.grad(val, c)[0].float()
+
+    dx, ds, dw = head_reference(head, x, grad)
+    for a, b in ((x.grad, dx), (head.norm.scale.grad, ds), (head.lm_head.w.grad, dw)):
+        compare(a.double().cpu().numpy(), b.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("cap,V,T", [(None, 1000, 1.0), ("tanh", 1000, 2.0), ("tanh", 2048, 1.0)])
+def test_teacher_head_to_student_head(cuda, cap, V, T):
+    """The distillation step as it is used: the teacher's head gives its top entries, the student's head
+    the loss and the gradients."""
+    teacher, x, g = make_head(cuda, 256, V, cap, 1)
+    student = make_head(cuda, 256, V, cap, 2)[0]
+    mask = torch.rand((2, 48), generator=g, device=cuda) > 0.2
+    with torch.no_grad():
+        top = teacher.token_logprobs(x, top_k=16, entropy=False, mask=mask)
+    x = x.requires_grad_(True)
+    loss = student.distillation_loss(x, top.top_ids, top.top_logprobs, temperature=T, mask=mask)
+    assert loss.shape == (2, 48) and (loss[~mask] == 0).all()
+    loss.sum().backward()
+    ids = top.top_ids.clamp(min=0)
+    q = torch.softmax(torch.where(mask[..., None], top.top_logprobs, 0.0).double() / T, -1)
+
+    def value(c):
+        lp = torch.log_softmax(c.double() / T, -1)
+        return ((q * (q.log() - lp.gather(2, ids))).sum(-1) * mask)
+
+    with torch.no_grad():
+        logits = plain_logits(student, x)
+        ref = value(logits)
+    assert logits.abs().max() < 16
+    assert (loss.double() - ref).abs().max() <= LOGIT / T
+
+    def grad(c):
+        c = c.double().requires_grad_(True)
+        return torch.autograd.grad(value(c).sum(), c)[0].float()
+
+    dx, ds, dw = head_reference(student, x, grad)
+    for a, b in ((x.grad, dx), (student.norm.scale.grad, ds), (student.lm_head.w.grad, dw)):
+        compare(a.double().cpu().numpy(), b.double().cpu().numpy())
+
+
+def test_head_gradient_kernel(cuda):
+    """Soft cap, amax and a padded pitch in the gradient kernel: dlogits against the formula, amax the
+    largest stored value, 0 where every row is masked."""
+    from macrogpt_jax_b200 import ops
+    T, V, Vp = 37, 1000, 1008
+    g = torch.Generator(device=cuda).manual_seed(7)
+    c = (15 * torch.tanh(torch.randn((T, Vp), generator=g, device=cuda) / 3)).bfloat16()
+    tok = torch.randint(0, V, (T,), generator=g, device=cuda)
+    mask = torch.rand(T, generator=g, device=cuda) > 0.5
+    adv = torch.randn(T, generator=g, device=cuda)
+    lg = c[:, :V]
+    stats = ops.token_logprobs_forward(lg, tok, mask, 0, 1.0, True, True)[4]
+    out = torch.full((T, Vp), 7.0, dtype=torch.bfloat16, device=cuda)
+    amax = torch.empty(1, device=cuda)
+    ops.token_logprobs_backward(lg, stats, tok, mask, 1.0, adv, None, None, None, (15.0, out, amax))
+    x = lg.double()
+    p = torch.softmax(x, -1)
+    cap = 1 - (x / 15) ** 2
+    one = torch.zeros_like(p).scatter_(1, tok[:, None], 1.0)
+    ref = (one - p) * adv.double()[:, None] * cap * mask[:, None]
+    # f32: p to 100 u, cap's two roundings relative to 1, the factor's three
+    tol = 2.0 ** -24 * adv.double().abs()[:, None] * (100 * p + 8 * one + 8 * (one - p).abs())
+    half = torch.finfo(torch.bfloat16).eps / 2
+    assert ((out[:, :V].double() - ref).abs() <= tol + half * ref.abs()).all()
+    assert (out[:, V:] == 7.0).all()
+    assert amax.item() == out[:, :V].abs().max().item()
+    none = torch.zeros(T, dtype=torch.bool, device=cuda)
+    ops.token_logprobs_backward(lg, stats, tok, none, 1.0, adv, None, None, None, (15.0, out, amax))
+    assert amax.item() == 0 and not out[:, :V].any()
+
+
+def test_head_retained_graph_and_changed_inputs(cuda):
+    """A second backward through a retained graph gives the same bits; a token changed in place after the
+    forward is noticed."""
+    head, x, g = make_head(cuda, 128, 512, "tanh", 5)
+    tok = torch.randint(0, 512, (2, 48), generator=g, device=cuda)
+    x = x.requires_grad_(True)
+    out = head.token_logprobs(x, tok)
+    a, = torch.autograd.grad(out.logprob.sum(), x, retain_graph=True)
+    b, = torch.autograd.grad(out.logprob.sum(), x, retain_graph=True)
+    assert torch.equal(a, b)
+    tok.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out.logprob.sum(), x)
+
+
+def test_generic_head(cuda):
+    """A head that is not fused (a norm without bf16 scale) takes the same calls."""
+    head, x, g = make_head(cuda, 128, 512, "tanh", 6)
+    head.norm.scale.data = head.norm.scale.data.float()
+    assert not head.fused()
+    tok = torch.randint(0, 512, (2, 48), generator=g, device=cuda)
+    x = x.requires_grad_(True)
+    out = head.token_logprobs(x, tok, top_k=4)
+    ref = torch.log_softmax(head.get_logits(x).double(), -1)
+    assert (out.logprob.double() - ref.gather(2, tok[..., None])[..., 0]).abs().max() <= 1e-4
+    loss = head.distillation_loss(x, out.top_ids, out.top_logprobs.detach())
+    (loss.sum() - out.logprob.sum()).backward()
+    assert x.grad.isfinite().all() and head.lm_head.w.grad.isfinite().all()

@@ -27,18 +27,20 @@ def fwd(r, tokens=P, token_bytes=8, k=0, lp=P, ent=P, top=None, ids=None, stats=
                                          ids, stats, None)
 
 
-def bwd(r, stats=P, tokens=P, token_bytes=8, dlp=P, dtop=None, ids=None, k=0, out=P, outer=400, inner=100):
+def bwd(r, stats=P, tokens=P, token_bytes=8, dlp=P, dtop=None, ids=None, k=0, cap=0.0, out=P, outer=400, inner=100,
+        amax=None):
     return C.load().ufp8_logprob_backward(ctypes.byref(r), stats, tokens, token_bytes, dlp, 1, None, 0, dtop, ids, k,
-                                          out, outer, inner, None)
+                                          cap, out, outer, inner, amax, None)
 
 
 def dfwd(r, ids=P, id_bytes=8, teacher=P, dtype=C.OUT_F32, k=4, loss=P, stats=None):
     return C.load().ufp8_distill_forward(ctypes.byref(r), ids, id_bytes, teacher, dtype, k, loss, stats, None)
 
 
-def dbwd(r, stats=P, ids=P, id_bytes=8, teacher=P, dtype=C.OUT_F32, k=4, dloss=P, out=P, outer=400, inner=100):
-    return C.load().ufp8_distill_backward(ctypes.byref(r), stats, ids, id_bytes, teacher, dtype, k, dloss, 1, out,
-                                          outer, inner, None)
+def dbwd(r, stats=P, ids=P, id_bytes=8, teacher=P, dtype=C.OUT_F32, k=4, dloss=P, cap=0.0, out=P, outer=400,
+         inner=100, amax=None):
+    return C.load().ufp8_distill_backward(ctypes.byref(r), stats, ids, id_bytes, teacher, dtype, k, dloss, 1, cap,
+                                          out, outer, inner, amax, None)
 
 
 @pytest.mark.parametrize("call,code,msg", [
@@ -73,6 +75,12 @@ def dbwd(r, stats=P, ids=P, id_bytes=8, teacher=P, dtype=C.OUT_F32, k=4, dloss=P
     (lambda: bwd(rows(), tokens=None), C.ERR_INVALID, "null tokens"),
     (lambda: bwd(rows(), dtop=P, k=3), C.ERR_INVALID, "null top_ids"),
     (lambda: bwd(rows(), dtop=P, ids=P, k=0), C.ERR_INVALID, "null top_ids"),
+    (lambda: bwd(rows(), cap=-1.0), C.ERR_INVALID, "cap must be"),
+    (lambda: bwd(rows(), cap=float("inf")), C.ERR_INVALID, "cap must be"),
+    (lambda: bwd(rows(dtype=C.OUT_F32), cap=15.0), C.ERR_UNSUPPORTED, "bf16"),
+    (lambda: bwd(rows(), amax=P + 2), C.ERR_ALIGN, "amax"),
+    (lambda: dbwd(rows(dtype=C.OUT_F32), amax=P), C.ERR_UNSUPPORTED, "bf16"),
+    (lambda: dbwd(rows(), cap=float("nan")), C.ERR_INVALID, "cap must be"),
     (lambda: dfwd(rows(), k=-1), C.ERR_INVALID, "entries must be"),
     (lambda: dfwd(rows(), k=1025), C.ERR_INVALID, "entries must be"),
     (lambda: dfwd(rows(), dtype=9), C.ERR_INVALID, "teacher_dtype 9"),
