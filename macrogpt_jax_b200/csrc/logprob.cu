@@ -1239,7 +1239,7 @@ int check_out(const ufp8_logit_rows* x, int64_t outer, int64_t inner, const char
 }
 
 template <class T, int kThr, int kMode, int kAhead>
-int launch_stat(StatArgs& a, int part_bits, cudaStream_t s) {
+int launch_stat(StatArgs& a, int part_bits, const DeviceInfo& dev, cudaStream_t s) {
   a.part_bits = part_bits;
   a.cap = 2 * a.k;
   cudaLaunchConfig_t cfg{};
@@ -1255,19 +1255,18 @@ int launch_stat(StatArgs& a, int part_bits, cudaStream_t s) {
   cfg.attrs = &attr;
   cfg.numAttrs = part_bits ? 1 : 0;
   static thread_local int smem_dev = -1;  // more than 48 KB of dynamic shared memory is asked for once per device
-  int cur = 0;
-  cudaError_t e = cudaGetDevice(&cur);
-  if (e == cudaSuccess && kMode == kTopK && smem_dev != cur) {
+  cudaError_t e = cudaSuccess;
+  if (kMode == kTopK && smem_dev != dev.device) {
     e = cudaFuncSetAttribute(rowstat_kernel<T, kThr, kMode, kAhead>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(TopLayout<kThr>::kBytes + sizeof(uint64_t) * 2 * kMaxTop * kMaxParts));
-    smem_dev = cur;
+    if (e == cudaSuccess) smem_dev = dev.device;
   }
   if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, rowstat_kernel<T, kThr, kMode, kAhead>, a);
   return e == cudaSuccess ? UFP8_OK : cuda_error(e, "row statistics launch");
 }
 
 template <class T, int kMode>
-int launch_stat(StatArgs& a, cudaStream_t s) {
+int launch_stat(StatArgs& a, const DeviceInfo& dev, cudaStream_t s) {
   constexpr int kTile = 256 * kUnits * T::kElems;  // columns
   // Few rows: a row is split as long as its parts are whole tiles and all CTAs run at once (those that
   // search for alternatives take more of an SM).
@@ -1276,17 +1275,19 @@ int launch_stat(StatArgs& a, cudaStream_t s) {
   while (bits < 3 && (a.r.rows << (bits + 1)) <= most && (static_cast<int64_t>(a.r.V) >> bits) > kTile) ++bits;
   // Many short rows: smaller CTAs, more of which are resident, hide each other's ends.
   if (a.r.rows >= 592) {
-    if (a.r.V <= 8192 && a.k <= 64) return launch_stat<T, 64, kMode, 1>(a, 0, s);
-    if (a.r.V <= (kMode == kTopK ? 32768 : 16384) && a.k <= 128) return launch_stat<T, 128, kMode, 1>(a, 0, s);
+    if (a.r.V <= 8192 && a.k <= 64) return launch_stat<T, 64, kMode, 1>(a, 0, dev, s);
+    // with alternatives also where the rows are one wave of 128 threads each (777 x 50257 f32: 40 -> 35 us)
+    if (a.k <= 128 && a.r.V <= (kMode == kTopK ? (a.r.rows <= 1184 ? a.r.V : 32768) : 16384))
+      return launch_stat<T, 128, kMode, 1>(a, 0, dev, s);
   }
   // Two tiles of loads in flight take twice the registers: where two CTAs per SM are all there are.
-  return (a.r.rows << bits) <= 296 ? launch_stat<T, 256, kMode, 2>(a, bits, s)
-                                   : launch_stat<T, 256, kMode, 1>(a, bits, s);
+  return (a.r.rows << bits) <= 296 ? launch_stat<T, 256, kMode, 2>(a, bits, dev, s)
+                                   : launch_stat<T, 256, kMode, 1>(a, bits, dev, s);
 }
 
 template <int kMode>
-int launch_stat(StatArgs& a, int dtype, cudaStream_t s) {
-  return dtype == UFP8_OUT_F32 ? launch_stat<F32, kMode>(a, s) : launch_stat<Bf16, kMode>(a, s);
+int launch_stat(StatArgs& a, int dtype, const DeviceInfo& dev, cudaStream_t s) {
+  return dtype == UFP8_OUT_F32 ? launch_stat<F32, kMode>(a, dev, s) : launch_stat<Bf16, kMode>(a, dev, s);
 }
 
 template <class T, bool kDistill, bool kHead>
@@ -1377,8 +1378,8 @@ extern "C" int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens
   a.top_id = top_ids;
   a.stats = reinterpret_cast<float4*>(stats);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (top_k > 0) return launch_stat<kTopK>(a, x->dtype, s);
-  return entropy ? launch_stat<kEntropy>(a, x->dtype, s) : launch_stat<kPlain>(a, x->dtype, s);
+  if (top_k > 0) return launch_stat<kTopK>(a, x->dtype, *dev, s);
+  return entropy ? launch_stat<kEntropy>(a, x->dtype, *dev, s) : launch_stat<kPlain>(a, x->dtype, *dev, s);
 }
 
 extern "C" int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const void* tokens,
@@ -1457,7 +1458,7 @@ extern "C" int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teache
   a.loss = loss;
   a.stats = reinterpret_cast<float4*>(stats);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return launch_stat<kTeacher>(a, x->dtype, s);
+  return launch_stat<kTeacher>(a, x->dtype, *dev, s);
 }
 
 extern "C" int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stats, const void* teacher_ids,

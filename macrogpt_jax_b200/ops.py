@@ -556,7 +556,7 @@ def _launch_on(t: torch.Tensor, kind: str, passes: float, fn) -> None:
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
             return _launch_on(t, kind, passes, fn)
-    stream = torch.cuda.current_stream(index).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(index)  # current_stream(index).cuda_stream in a tenth of its time
     if _timer is None:
         fn(stream)
     else:
@@ -615,7 +615,8 @@ def token_logprobs_forward(logits: torch.Tensor, tokens: torch.Tensor | None, ma
     """(logprob, entropy, top log probabilities, top ids) over the logits' leading shape, then the
     backward's stats; None where not asked for (ufp8_logprob_forward)."""
     lr = logit_rows(logits)
-    t, lead, dev, f32 = lr.logits, logits.shape[:-1], logits.device, torch.float32
+    t, dev, f32 = lr.logits, logits.device, torch.float32
+    lead = logits.shape[:-1]
     lp = torch.empty_like(tokens, dtype=f32) if tokens is not None else None
     ent = (_empty_f32(lead, dev) if lp is None else torch.empty_like(lp)) if entropy else None
     top_id = torch.empty(*lead, top_k, dtype=torch.int64, device=dev) if top_k else None
