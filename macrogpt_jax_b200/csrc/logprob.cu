@@ -24,7 +24,7 @@
 namespace ufp8 {
 namespace {
 
-constexpr int kThreads = 256;  // of a gradient CTA; a statistics CTA has 256 or 64
+constexpr int kThreads = 256;  // of a gradient CTA; a statistics CTA has 256, 128 or 64
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 256;
 constexpr int kMaxEntries = 1024;   // teacher entries of a row
@@ -335,7 +335,8 @@ struct TopShared {
   uint32_t hist[256];
   uint32_t maxima[kThr];  // order16 of a thread's maximum over the even / odd slots of the table
   uint32_t reached;       // order16 that at least k elements of the CTA's columns reach (0: not known)
-  int items, n, n_last;   // entries of the item list, gathered keys, keys in `last`
+  int items, n;        // entries of the item list, gathered keys
+  int n_last, pushed;  // keys in `last`, keys brought to the first CTA
   int bin, above, in_bin;
   float m, ls;
   alignas(16) uint64_t last[kFinal];
@@ -551,7 +552,8 @@ struct StatArgs {
 };
 
 __device__ __forceinline__ float teacher_val(const StatArgs& a, int64_t i) {
-  return a.teacher_f32 ? static_cast<const float*>(a.teacher)[i] : Bf16::to_f(static_cast<const uint16_t*>(a.teacher)[i]);
+  return a.teacher_f32 ? static_cast<const float*>(a.teacher)[i]
+                       : Bf16::to_f(static_cast<const uint16_t*>(a.teacher)[i]);
 }
 // A teacher entry: its column's logit (NaN: an id past the last column) and the teacher's value there.
 struct Entry {
@@ -646,14 +648,14 @@ __device__ __noinline__ int search_row(const Row<T>& x, int u_begin, int u_end, 
 }
 
 // The k largest of the CTA's units [u_begin, u_end), and a few more, as keys: this warp's list (*mine, *n_mine);
-// returns the number of all warps.  `reached` is a bound that k of the elements reach, `best` the thread's
-// maximum.  The table says which thread and which tiles saw a maximum that reaches it; those (little more
-// than k) are read once more, each by one thread.  Where too many elements equal the bound (a constant
-// row, say), the row is searched as a whole.
+// returns the number of all warps.  *all: the lists one after another (null: they are apart).  `reached` is a
+// bound that k of the elements reach, `best` the thread's maximum.  The table says which thread and which
+// tiles saw a maximum that reaches it; those (little more than k) are read once more, each unit by one
+// thread.  Where too many elements equal the bound (a constant row, say), the row is searched as a whole.
 template <class T, int kThr>
 __device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end, int per_slot, int slots, uint32_t best,
                                         int k, int ib, char* mem, TopShared<kThr>& sh, const uint64_t** mine,
-                                        int* n_mine) {
+                                        int* n_mine, const uint64_t** all) {
   using L = TopLayout<kThr>;
   constexpr int kTile = kThr * kUnits;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -719,8 +721,10 @@ __device__ __forceinline__ int find_top(const Row<T>& x, int u_begin, int u_end,
     const int per = (n + kThr / 32 - 1) / (kThr / 32);
     *mine = gather + warp * per;
     *n_mine = max(0, min(per, n - warp * per));
+    *all = gather;
     return n;
   }
+  *all = nullptr;
   __syncthreads();  // the table, the items and the gathered keys give way to the regions
   uint64_t* region = reinterpret_cast<uint64_t*>(mem) + warp * kRegion;
   *mine = region;
@@ -826,7 +830,7 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kKeyBits > 1
   int slot = 0, in_slot = 0;
   uint32_t best[2] = {0, 0}, order = 0;
 
-  if (kTop && tid == 0) sh.items = sh.n = sh.n_last = 0;
+  if (kTop && tid == 0) sh.items = sh.n = sh.n_last = sh.pushed = 0;
 
   for (int first = u_begin; first < u_end; first += kAhead * kTile) {
     Unit<T> w[kAhead][kUnits];
@@ -865,7 +869,7 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kKeyBits > 1
     st = tid < kNWarps ? sh_stat[tid] : Stat{kNegInf, 0.0f, 0.0f};
     st = warp_merge(st, c2);
   }
-  const uint64_t* mine = nullptr;
+  const uint64_t *mine = nullptr, *all = nullptr;
   int n_mine = 0, n = 0;
   const int bits = T::kKeyBits + a.ib;
   uint64_t bound = 0;
@@ -875,7 +879,8 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kKeyBits > 1
       if ((tid & 31) == 0) sh.reached = r;
     }
     __syncthreads();
-    n = find_top<T, kThr>(x, u_begin, u_end, per_slot, slot, max(best[0], best[1]), a.k, a.ib, mem, sh, &mine, &n_mine);
+    n = find_top<T, kThr>(x, u_begin, u_end, per_slot, slot, max(best[0], best[1]), a.k, a.ib, mem, sh, &mine, &n_mine,
+                          &all);
   }
 
   if (n_parts > 1) {
@@ -890,13 +895,11 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kKeyBits > 1
         __syncthreads();
         if (tid == 0) sh.n_last = 0;
       }
-      if (tid == 0) sh.n = 0;
-      __syncthreads();
     }
     cluster.barrier_wait();
     if constexpr (kTop) {
       uint64_t* to = cluster.map_shared_rank(part_keys + part * a.cap, 0);
-      for (int i = tid & 31; i < n_mine; i += 32) to[atomicAdd(&sh.n, 1)] = mine[i];
+      for (int i = tid & 31; i < n_mine; i += 32) to[atomicAdd(&sh.pushed, 1)] = mine[i];
     }
     if (tid == 0) {
       PartsShared* to = cluster.map_shared_rank(&parts, 0);
@@ -943,9 +946,9 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kKeyBits > 1
     }
   }
   if constexpr (kTop) {
-    // V >= k: there are k keys at least.  The keys of one CTA that are not many lie one after another.
-    const uint64_t* last = mine - warp * ((n + kNWarps - 1) / kNWarps);
-    if (n_parts > 1 || n > kFinal) {
+    // V >= k: there are k keys at least.  One CTA's keys, if they are not many, are compared where they are.
+    const uint64_t* last = all;
+    if (n_parts > 1 || n > kFinal || all == nullptr) {
       n = collect<kThr>(mine, n_mine, n, a.k, kFinal, bound, bits, sh);
       last = sh.last;
     } else {
@@ -1201,8 +1204,9 @@ int rows_args(const ufp8_logit_rows* x, RowsArgs* a, const char* who) {
   if (x->dtype != UFP8_OUT_BF16 && x->dtype != UFP8_OUT_F32)
     return set_error(UFP8_ERR_INVALID, "%s: dtype %d is not UFP8_OUT_BF16/UFP8_OUT_F32", who, x->dtype);
   if (x->rows < 0 || x->V < 1) return set_error(UFP8_ERR_INVALID, "%s: rows must be >= 0 and V >= 1", who);
-  if (x->rows >= (int64_t(1) << 31)) return set_error(UFP8_ERR_INVALID, "%s: rows exceed 2^31", who);
-  if (x->V >= (int64_t(1) << 31) - (int64_t(1) << 20)) return set_error(UFP8_ERR_INVALID, "%s: V exceeds 2^31", who);
+  const int64_t most = (int64_t(1) << 31) - (int64_t(1) << 20);  // an index past the end still fits 32 bits
+  if (x->rows >= most) return set_error(UFP8_ERR_INVALID, "%s: rows exceed 2^31", who);
+  if (x->V >= most) return set_error(UFP8_ERR_INVALID, "%s: V exceeds 2^31", who);
   if (x->rows > 0 && x->inner < 1) return set_error(UFP8_ERR_INVALID, "%s: inner must be >= 1", who);
   if (!(x->temperature > 0.0f) || std::isinf(x->temperature))
     return set_error(UFP8_ERR_INVALID, "%s: temperature must be finite and > 0", who);
@@ -1476,7 +1480,8 @@ extern "C" int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stat
   if (!al(dlogits, x->dtype == UFP8_OUT_F32 ? 4 : 2))
     return set_error(UFP8_ERR_ALIGN, "%s: dlogits not aligned to their type", who);
   if (x->rows == 0 && !amax) return UFP8_OK;
-  if (x->rows > 0 && (!stats || !dlogits || !dloss)) return set_error(UFP8_ERR_INVALID, "%s: null stats, dloss or dlogits", who);
+  if (x->rows > 0 && (!stats || !dlogits || !dloss))
+    return set_error(UFP8_ERR_INVALID, "%s: null stats, dloss or dlogits", who);
   DeviceInfo* dev;
   if (int rc = device_info(&dev)) return rc;
   a.stats = reinterpret_cast<const float4*>(stats);

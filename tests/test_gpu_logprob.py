@@ -136,6 +136,31 @@ def test_top_orders(cuda, dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [3, 210, 700])
+@pytest.mark.parametrize("count", [900, 1300, 2600])
+def test_top_ties_in_one_warp(cuda, dtype, rows, count):
+    """More equal maxima than the gathered keys hold, all of them in columns that one warp of a CTA reads:
+    the search of the whole row then leaves few keys, in one warp's list."""
+    from macrogpt_jax_b200.logprobs import token_logprobs
+    V = 50000 if rows < 700 else 20000
+    per = 8 if dtype == torch.bfloat16 else 4
+    threads = 256 if rows < 592 else 128
+    col = torch.arange(V, device=cuda)
+    warp0 = col // per % threads < 32
+    g = torch.Generator(device=cuda).manual_seed(rows + count)
+    x = torch.randn((rows, V), generator=g, device=cuda)
+    x[:, col[warp0][:count]] = 9.0
+    x = x.to(dtype)
+    tok = torch.randint(0, V, (rows,), generator=g, device=cuda)
+    for k in (1, 7, 100):
+        check_score(x[:3], tok[:3], take(token_logprobs(x, tok, top_k=k), slice(0, 3)), 1.0, k)
+
+
+def take(out, rows):
+    return type(out)(*(t[rows] for t in out))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_score_not_finite(cuda, dtype):
     """+inf, NaN and rows of only -inf give NaN, and only in their own row; the order stays defined."""
     from macrogpt_jax_b200.logprobs import token_logprobs
@@ -149,8 +174,7 @@ def test_score_not_finite(cuda, dtype):
         assert torch.equal(torch.isnan(t), torch.tensor([0, 1, 1, 1, 1, 0], device=cuda).bool())
     assert torch.equal(out.top_ids, torch.from_numpy(top_ref(x, 30)).to(cuda))
     good = torch.tensor([0, 5], device=cuda)
-    check_score(x[good], tok[good], token_logprobs(x, tok, top_k=30).__class__(
-        *(t[good] for t in out)), 1.0, 30)
+    check_score(x[good], tok[good], take(out, good), 1.0, 30)
 
 
 def test_score_tokens_and_mask(cuda):
@@ -309,8 +333,11 @@ def test_score_gradient_by_differences(cuda):
     V, T, eps = 9, 0.8, 2.0 ** -6
     x, _, g = make(cuda, 1, V, torch.float32, 4, 1.0)
     tok = torch.tensor([4], device=cuda)
-    f = lambda t: (lambda o: 1.5 * o.logprob[..., None] - 0.7 * o.entropy[..., None] + o.top_logprobs[..., 1:2])(  # noqa: E731
-        token_logprobs(t, tok.expand(t.shape[0]), top_k=2, temperature=T))
+
+    def f(t):
+        o = token_logprobs(t, tok.expand(t.shape[0]), top_k=2, temperature=T)
+        return 1.5 * o.logprob[..., None] - 0.7 * o.entropy[..., None] + o.top_logprobs[..., 1:2]
+
     xg = x.clone().requires_grad_(True)
     got, = torch.autograd.grad(f(xg).sum(), xg)
     pts = torch.cat([x + eps * torch.eye(V, device=cuda), x - eps * torch.eye(V, device=cuda)])
