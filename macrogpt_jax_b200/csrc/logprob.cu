@@ -284,13 +284,14 @@ __device__ __forceinline__ void fold_tile(const Unit<T> (&w)[kUnits], float cm, 
 // A key orders an element by value (NaN above all, -0 equal to 0) and then by column, lower first:
 // the value's bits mapped to an unsigned order, above ib bits of (2^ib - 1 - column).  Keys of a row
 // are distinct, so the k largest are one set whatever the order in which they were found.
+__device__ __forceinline__ uint32_t value_order(float x) {
+  uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));  // one zero
+  b ^= static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u;
+  return x != x ? 0xFFFFFFFFu : b;
+}
 template <class T>
 __device__ __forceinline__ uint64_t make_key(float x, uint32_t col, int ib) {
-  uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));  // one zero
-  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  if (x != x) b = 0xFFFFFFFFu;
-  b >>= 32 - T::kKeyBits;
-  return (static_cast<uint64_t>(b) << ib) | (((1ull << ib) - 1ull) - col);
+  return (static_cast<uint64_t>(value_order(x) >> (32 - T::kKeyBits)) << ib) | (((1ull << ib) - 1ull) - col);
 }
 template <class T>
 __device__ __forceinline__ float key_value(uint64_t key, int ib) {
@@ -307,10 +308,7 @@ __device__ __forceinline__ float order_value(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
 // The upper 16 bits of x's order.
-template <class T>
-__device__ __forceinline__ uint32_t order16(float x) {
-  return static_cast<uint32_t>(make_key<T>(x, 0, 1) >> (T::kKeyBits - 16 + 1));
-}
+__device__ __forceinline__ uint32_t order16(float x) { return value_order(x) >> 16; }
 
 constexpr int kRegion = 512;  // candidate keys of a warp; at least kMaxTop + the 256 columns of a warp's units
 constexpr int kSlots = 32;    // entries per thread of the table of maxima
@@ -846,7 +844,7 @@ __global__ void __launch_bounds__(kThr, min_ctas(kMode == kTopK, T::kKeyBits > 1
       for (int u = 1; u < kUnits; ++u) cm = maxn(cm, unit_max<T>(w[h][u]));
       fold_tile<T, kEnt>(w[h], cm, st, c2);
       if constexpr (kTop) {
-        order = max(order, order16<T>(cm));
+        order = max(order, order16(cm));
         if (++in_slot == per_slot || u0 + kTile >= u_end) {
           table[slot * kThr + tid] = static_cast<uint16_t>(order);
           if (slot & 1)
