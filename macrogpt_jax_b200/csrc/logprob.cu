@@ -1274,24 +1274,33 @@ int launch_stat(StatArgs& a, int part_bits, const DeviceInfo& dev, cudaStream_t 
   return e == cudaSuccess ? UFP8_OK : cuda_error(e, "row statistics launch");
 }
 
+// CTAs of a row and threads of a CTA, by rows per SM and the row's length (us with 256 threads / as chosen, entropy
+// or 20 alternatives, on 148 SMs).
 template <class T, int kMode>
 int launch_stat(StatArgs& a, const DeviceInfo& dev, cudaStream_t s) {
+  constexpr bool kTop = kMode == kTopK, kF32 = T::kKeyBits > 16;
   constexpr int kTile = 256 * kUnits * T::kElems;  // columns
-  // Few rows: a row is split as long as its parts are whole tiles and all CTAs run at once (those that
-  // search for alternatives take more of an SM).
-  const int64_t most = kMode == kTopK ? 400 : 800;
+  const int64_t rows = a.r.rows, V = a.r.V, sm = dev.sm_count, tiles = V / kTile;
+  // Few rows: a row is split as long as its parts are whole tiles and all CTAs run at once (those that search for
+  // alternatives take more of an SM).  1 x 128256: 11.7 / 3.7; 48: 12.2 / 5.7; 148: 12.4 / 10.9; 300: 21 / 19.
   int bits = 0;
-  while (bits < 3 && (a.r.rows << (bits + 1)) <= most && (static_cast<int64_t>(a.r.V) >> bits) > kTile) ++bits;
-  // Many short rows: smaller CTAs, more of which are resident, hide each other's ends.
-  if (a.r.rows >= 592) {
-    if (a.r.V <= 8192 && a.k <= 64) return launch_stat<T, 64, kMode, 1>(a, 0, dev, s);
-    // with alternatives also where the rows are one wave of 128 threads each (777 x 50257 f32: 40 -> 35 us)
-    if (a.k <= 128 && a.r.V <= (kMode == kTopK ? (a.r.rows <= 1184 ? a.r.V : 32768) : 16384))
-      return launch_stat<T, 128, kMode, 1>(a, 0, dev, s);
+  while (bits < 3 && (rows << (bits + 1)) <= (kTop ? 27 * sm / 10 : 11 * sm / 2) && (V >> bits) > kTile) ++bits;
+  // Long rows whose halves still balance better.  600 x 128256: 35.6 / 32.4; 1055: 52.8 / 50.9; 1300 would lose.
+  if (!kTop && bits == 0 && rows <= 15 * sm / 2 && tiles >= 14) bits = 1;
+  if (rows >= 4 * sm) {
+    // Many short rows: smaller CTAs, more of which are resident, hide each other's ends.  8000 x 1500: 29 / 12.8,
+    // with alternatives 88 / 31.
+    if (V <= 8192 && a.k <= 64) return launch_stat<T, 64, kMode, 1>(a, 0, dev, s);
+    // The same for longer ones (6000 x 32000 with alternatives: 107 / 95), and where the rows are more than one wave of
+    // 256 threads each but not of 128 (1055 x 50257 f32: 41.8 / 36.1; 900 x 128256 with alternatives: 59 / 56).
+    const bool shorter = V <= (kTop ? (kF32 ? 65536 : 32768) : 16384);
+    const bool one_wave = kTop ? rows > (kF32 ? 4 : 5) * sm && rows <= 8 * sm
+                               : rows > 6 * sm && rows <= 12 * sm && tiles >= 8 && tiles < 14;
+    if (a.k <= 128 && (shorter || one_wave)) return launch_stat<T, 128, kMode, 1>(a, 0, dev, s);
   }
   // Two tiles of loads in flight take twice the registers: where two CTAs per SM are all there are.
-  return (a.r.rows << bits) <= 296 ? launch_stat<T, 256, kMode, 2>(a, bits, dev, s)
-                                   : launch_stat<T, 256, kMode, 1>(a, bits, dev, s);
+  return (rows << bits) <= 2 * sm ? launch_stat<T, 256, kMode, 2>(a, bits, dev, s)
+                                  : launch_stat<T, 256, kMode, 1>(a, bits, dev, s);
 }
 
 template <int kMode>

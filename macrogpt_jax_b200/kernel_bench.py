@@ -3,7 +3,7 @@
     python -m macrogpt_jax_b200.kernel_bench [--tokens T] [--d D] [--hidden H]
                                              [--gemms F1,F2,B2,B1,B4,B3] [--reps R] [--warmup W]
                                              [--variant V] [--seconds S] [--cublas]
-                                             [--quant | --norm | --rs-push | --xent | --ns |
+                                             [--quant | --norm | --rs-push | --xent | --logprob | --ns |
                                               --attn [--batch B --seq S --kv-heads H --group I]]
 
 Each named GEMM of the GMLP step runs R times after W warm-up launches on seeded fp8
@@ -240,6 +240,35 @@ def xent_bench(args, dev):
     print(json.dumps({"tokens": T, "vocab": V, **res}), flush=True)
 
 
+def logprob_bench(args, dev):
+    """The kernels of token_logprobs and topk_distillation_loss on [tokens, vocab] logits (--f32: f32
+    logits; default bf16): forward (logits read once) alone, with the entropy, with --top-k
+    alternatives and against --top-k teacher entries, and the gradients (read once, written once);
+    algorithmic GB/s."""
+    T, V, k = args.tokens, args.vocab, args.top_k
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(7)
+    x = (torch.randn((T, V), generator=gen, device=dev) * 3).to(torch.float32 if args.f32 else torch.bfloat16)
+    tok = torch.randint(0, V, (T,), generator=gen, device=dev)
+    ids = torch.randint(0, V, (T, k), generator=gen, device=dev)
+    teacher = torch.randn((T, k), generator=gen, device=dev)
+    d = torch.randn((T,), generator=gen, device=dev)
+    stats = ops.token_logprobs_forward(x, tok, None, 0, 1.0, True, True)[4]
+    dstats = ops.distill_forward(x, ids, teacher, None, 1.0, True)[1]
+    n = T * V * x.element_size()
+    res = {}
+    for kind, fn, nbytes in (
+            ("logprob", lambda: ops.token_logprobs_forward(x, tok, None, 0, 1.0, False, False), n),
+            ("logprob_entropy", lambda: ops.token_logprobs_forward(x, tok, None, 0, 1.0, True, False), n),
+            ("logprob_top", lambda: ops.token_logprobs_forward(x, tok, None, k, 1.0, True, False), n),
+            ("distill", lambda: ops.distill_forward(x, ids, teacher, None, 1.0, True), n),
+            ("logprob_grad", lambda: ops.token_logprobs_backward(x, stats, tok, None, 1.0, d, d, None, None), 2 * n),
+            ("distill_grad", lambda: ops.distill_backward(x, dstats, ids, teacher, None, 1.0, d), 2 * n)):
+        us = _time_us(fn, args.reps, args.warmup)
+        res[kind] = {"us": us, "gbs": nbytes / us / 1e3}
+    print(json.dumps({"tokens": T, "vocab": V, "top_k": k, "dtype": "f32" if args.f32 else "bf16", **res}), flush=True)
+
+
 def ns_bench(args, dev):
     """Newton-Schulz (ufp8_newton_schulz) on [batch, d, hidden] f32 slices, 5 'muon' steps;
     algorithmic TF/s = 5 (4 s^2 l + 2 s^3) per slice / time."""
@@ -304,6 +333,10 @@ def main():
     ap.add_argument("--norm", action="store_true", help="time the RMSNorm kernels on [tokens, d] instead")
     ap.add_argument("--xent", action="store_true", help="time the cross-entropy kernels on [tokens, vocab] instead")
     ap.add_argument("--vocab", type=int, default=128256)
+    ap.add_argument("--logprob", action="store_true",
+                    help="time token_logprobs and topk_distillation_loss on [tokens, vocab] instead")
+    ap.add_argument("--top-k", type=int, default=64, help="alternatives and teacher entries (--logprob)")
+    ap.add_argument("--f32", action="store_true", help="f32 logits (--logprob)")
     ap.add_argument("--ns", action="store_true", help="time Newton-Schulz on [batch, d, hidden] instead")
     ap.add_argument("--batch", type=int, default=2)
     ap.add_argument("--attn", action="store_true",
@@ -326,6 +359,8 @@ def main():
         return norm_bench(args, dev)
     if args.xent:
         return xent_bench(args, dev)
+    if args.logprob:
+        return logprob_bench(args, dev)
     if args.ns:
         return ns_bench(args, dev)
     if args.attn:

@@ -7,6 +7,8 @@ merges (5 lanes + 7 warps, a few each; parts of a row add fewer).  So s is good 
 3 u E[|z|], and log p to that plus 6 u (|log p| + 1): z again, its fma and the product with ln 2.
 The entropy adds t = sum p z: (n + 72) u E|z| + 3 u E[z^2].  A gradient is p times a factor, p good to
 the error of log p plus 4 u, plus half a step of the output type.  All norms are taken per element."""
+import collections
+
 import numpy as np
 import pytest
 import torch
@@ -14,6 +16,9 @@ import torch
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
+
+
+TokenRows = collections.namedtuple("TokenRows", "logprob entropy top_logprobs top_ids")
 
 
 def chain(V):
@@ -100,6 +105,25 @@ def test_score_row_counts(cuda, rows):
     for V in (5000, 70001):
         x, tok, _ = make(cuda, rows, V, torch.bfloat16, rows)
         check_score(x, tok, token_logprobs(x, tok, top_k=33), 1.0, 33)
+
+
+@pytest.mark.parametrize("rows,V,dtype", [(900, 115001, torch.bfloat16), (1000, 70001, torch.bfloat16),
+                                          (900, 60001, torch.float32), (2000, 8192, torch.bfloat16),
+                                          (2000, 20001, torch.float32), (1200, 33001, torch.bfloat16)])
+def test_score_many_rows(cuda, rows, V, dtype):
+    """The choices of CTA size and parts for many rows (row starts at every alignment)."""
+    from macrogpt_jax_b200.distill import topk_distillation_loss
+    from macrogpt_jax_b200.logprobs import token_logprobs
+    x, tok, g = make(cuda, rows, V, dtype, rows)
+    some = torch.randperm(rows, generator=g, device=cuda)[:150]
+    for k in (0, 20, 100):
+        out = token_logprobs(x, tok, top_k=k)
+        check_score(x[some], tok[some], TokenRows(*(None if t is None else t[some] for t in out)), 1.0, k)
+    ids = torch.randint(0, V, (rows, 40), generator=g, device=cuda)
+    t = torch.randn((rows, 40), generator=g, device=cuda)
+    loss = topk_distillation_loss(x, ids, t)[some]
+    rl, ltol, *_ = distill_ref(x[some], ids[some], t[some], 1.0)
+    assert ((loss.double() - rl).abs() <= ltol).all()
 
 
 @pytest.mark.parametrize("k", [1, 2, 3, 4, 5, 8, 9, 16, 17, 64, 65, 128, 129, 255, 256])
