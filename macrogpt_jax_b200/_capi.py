@@ -325,36 +325,40 @@ def xent_backward(logits_ptr, rows, V, ldl, labels_ptr, mask_ptr, lse_ptr, qrow_
     _count((1 if fmt != BF16 else 0) + (1 if rows > 0 else 0))
 
 
-def logprob_forward(rows: LogitRows, tokens_ptr, token_bytes, top_k, logprob_ptr, entropy_ptr, top_lp_ptr, top_id_ptr,
-                    stats_ptr, stream) -> None:
+# The logit-row operators are called per sampled token: their entry points are looked up once and their
+# arguments passed on as they come (see the prototypes in include/ufp8.h).
+_entry = {}
+
+
+def _call(name: str, rows: LogitRows, args) -> None:
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(load(), name)
+    rc = fn(rows, *args)
+    if rc:
+        check(rc)
+    if rows.rows > 0:
+        _count(1)
+
+
+def logprob_forward(rows: LogitRows, *args) -> None:
     """ufp8_logprob_forward: log probabilities of given tokens, entropy and top alternatives."""
-    check(load().ufp8_logprob_forward(ctypes.byref(rows), tokens_ptr, token_bytes, top_k, logprob_ptr, entropy_ptr,
-                                      top_lp_ptr, top_id_ptr, stats_ptr, stream))
-    _count(1 if rows.rows > 0 else 0)
+    _call("ufp8_logprob_forward", rows, args)
 
 
-def logprob_backward(rows: LogitRows, stats_ptr, tokens_ptr, token_bytes, dlp_ptr, dlp_stride, dent_ptr, dent_stride,
-                     dtop_ptr, top_id_ptr, top_k, cap, out_ptr, out_outer, out_inner, amax_ptr, stream) -> None:
-    check(load().ufp8_logprob_backward(ctypes.byref(rows), stats_ptr, tokens_ptr, token_bytes, dlp_ptr, dlp_stride,
-                                       dent_ptr, dent_stride, dtop_ptr, top_id_ptr, top_k, cap, out_ptr, out_outer,
-                                       out_inner, amax_ptr, stream))
-    _count(1 if rows.rows > 0 else 0)
+def logprob_backward(rows: LogitRows, *args) -> None:
+    """ufp8_logprob_backward: the gradient of the above."""
+    _call("ufp8_logprob_backward", rows, args)
 
 
-def distill_forward(rows: LogitRows, ids_ptr, id_bytes, teacher_ptr, teacher_dtype, entries, loss_ptr, stats_ptr,
-                    stream) -> None:
+def distill_forward(rows: LogitRows, *args) -> None:
     """ufp8_distill_forward: the loss against a teacher's top logits."""
-    check(load().ufp8_distill_forward(ctypes.byref(rows), ids_ptr, id_bytes, teacher_ptr, teacher_dtype, entries,
-                                      loss_ptr, stats_ptr, stream))
-    _count(1 if rows.rows > 0 else 0)
+    _call("ufp8_distill_forward", rows, args)
 
 
-def distill_backward(rows: LogitRows, stats_ptr, ids_ptr, id_bytes, teacher_ptr, teacher_dtype, entries, dloss_ptr,
-                     dloss_stride, cap, out_ptr, out_outer, out_inner, amax_ptr, stream) -> None:
-    check(load().ufp8_distill_backward(ctypes.byref(rows), stats_ptr, ids_ptr, id_bytes, teacher_ptr, teacher_dtype,
-                                       entries, dloss_ptr, dloss_stride, cap, out_ptr, out_outer, out_inner, amax_ptr,
-                                       stream))
-    _count(1 if rows.rows > 0 else 0)
+def distill_backward(rows: LogitRows, *args) -> None:
+    """ufp8_distill_backward: the gradient of the above."""
+    _call("ufp8_distill_backward", rows, args)
 
 
 def newton_schulz_workspace(batch: int, m: int, n: int) -> int:

@@ -544,23 +544,27 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _id_bytes(t: torch.Tensor | None) -> int:
+    return 4 if t is not None and t.dtype == torch.int32 else 8
+
+
 def _empty_f32(shape, device) -> torch.Tensor:
     """torch.empty; sizes as separate integers take half the host time of a tuple of them."""
     return torch.empty(*(shape or ((),)), dtype=torch.float32, device=device)
 
 
-def _launch_on(t: torch.Tensor, kind: str, passes: float, fn) -> None:
-    """fn(stream) on the current stream of t's device, which may be another one than the current device;
-    `passes` over t's bytes are its work."""
+def _call_on(t: torch.Tensor, kind: str, passes: float, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of t's device, which may be another one than the current
+    device; `passes` over t's bytes are its work."""
     index = t.device.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            return _launch_on(t, kind, passes, fn)
+            return _call_on(t, kind, passes, fn, *args)
     stream = torch._C._cuda_getCurrentRawStream(index)  # current_stream(index).cuda_stream in a tenth of its time
     if _timer is None:
-        fn(stream)
+        fn(*args, stream)
     else:
-        _timer.wrap(kind, passes * t.element_size() * t.numel(), lambda: fn(stream))
+        _timer.wrap(kind, passes * t.element_size() * t.numel(), lambda: fn(*args, stream))
 
 
 def logit_rows(logits: torch.Tensor) -> LogitRows:
@@ -622,9 +626,8 @@ def token_logprobs_forward(logits: torch.Tensor, tokens: torch.Tensor | None, ma
     top_id = torch.empty(*lead, top_k, dtype=torch.int64, device=dev) if top_k else None
     top_lp = torch.empty_like(top_id, dtype=f32) if top_k else None
     stats = torch.empty(lr.rows, 4, dtype=f32, device=dev) if want_stats else None
-    _launch_on(t, "logprob", 1.0, lambda stream: C.logprob_forward(
-        lr.c(temperature, mask), _ptr(tokens), tokens.element_size() if tokens is not None else 0, top_k, _ptr(lp),
-        _ptr(ent), _ptr(top_lp), _ptr(top_id), _ptr(stats), stream))
+    _call_on(t, "logprob", 1.0, C.logprob_forward, lr.c(temperature, mask), _ptr(tokens), _id_bytes(tokens), top_k,
+             _ptr(lp), _ptr(ent), _ptr(top_lp), _ptr(top_id), _ptr(stats))
     return lp, ent, top_lp, top_id, stats
 
 
@@ -653,10 +656,9 @@ def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: t
     dtop = None if dtop is None else dtop.to(torch.float32).contiguous()
     top_k = top_id.shape[-1] if dtop is not None else 0
     cap, out, outer, inner, amax_t = _grad_target(lr, head)
-    _launch_on(t, "logprob_grad", 2.0, lambda stream: C.logprob_backward(
-        lr.c(temperature, mask), stats.data_ptr(), _ptr(tokens), tokens.element_size() if tokens is not None else 0,
-        _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, cap, out.data_ptr(), outer, inner,
-        _ptr(amax_t), stream))
+    _call_on(t, "logprob_grad", 2.0, C.logprob_backward, lr.c(temperature, mask), stats.data_ptr(), _ptr(tokens),
+             _id_bytes(tokens), _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, cap,
+             out.data_ptr(), outer, inner, _ptr(amax_t))
     return out
 
 
@@ -667,9 +669,8 @@ def distill_forward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tens
     t = lr.logits
     loss = _empty_f32(logits.shape[:-1], t.device)
     stats = torch.empty(lr.rows, 4, dtype=torch.float32, device=t.device) if want_stats else None
-    _launch_on(t, "distill", 1.0, lambda stream: C.distill_forward(
-        lr.c(temperature, mask), ids.data_ptr(), ids.element_size(), teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype],
-        ids.shape[-1], loss.data_ptr(), _ptr(stats), stream))
+    _call_on(t, "distill", 1.0, C.distill_forward, lr.c(temperature, mask), ids.data_ptr(), _id_bytes(ids),
+             teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], loss.data_ptr(), _ptr(stats))
     return loss, stats
 
 
@@ -681,10 +682,9 @@ def distill_backward(logits: torch.Tensor, stats: torch.Tensor, ids: torch.Tenso
     t = lr.logits
     dloss, stride = _row_grad(dloss)
     cap, out, outer, inner, amax_t = _grad_target(lr, head)
-    _launch_on(t, "distill_grad", 2.0, lambda stream: C.distill_backward(
-        lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(), ids.element_size(), teacher.data_ptr(),
-        _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride, cap, out.data_ptr(), outer, inner,
-        _ptr(amax_t), stream))
+    _call_on(t, "distill_grad", 2.0, C.distill_backward, lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(),
+             _id_bytes(ids), teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride,
+             cap, out.data_ptr(), outer, inner, _ptr(amax_t))
     return out
 
 
