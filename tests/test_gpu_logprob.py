@@ -109,7 +109,8 @@ def test_score_row_counts(cuda, rows):
 
 @pytest.mark.parametrize("rows,V,dtype", [(900, 115001, torch.bfloat16), (1000, 70001, torch.bfloat16),
                                           (900, 60001, torch.float32), (2000, 8192, torch.bfloat16),
-                                          (2000, 20001, torch.float32), (1200, 33001, torch.bfloat16)])
+                                          (2000, 20001, torch.float32), (1200, 33001, torch.bfloat16),
+                                          (420, 300001, torch.bfloat16), (800, 270001, torch.bfloat16)])
 def test_score_many_rows(cuda, rows, V, dtype):
     """The choices of CTA size and parts for many rows (row starts at every alignment)."""
     from macrogpt_jax_b200.distill import topk_distillation_loss
@@ -157,6 +158,16 @@ def test_top_orders(cuda, dtype, rows):
         tok = torch.full((xi.shape[0],), V - 1, device=cuda)
         for k in (1, 20, 200):
             check_score(xi, tok, token_logprobs(xi, tok, top_k=k), 1.0, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale,T", [(1e30, 0.5), (1e-30, 1.0), (2.5, 0.01), (2.5, 1e4), (40.0, 1.0)])
+def test_score_magnitudes(cuda, dtype, scale, T):
+    """Logits so large that the others have no weight, so small that all have the same, and temperatures
+    that do either."""
+    from macrogpt_jax_b200.logprobs import token_logprobs
+    x, tok, _ = make(cuda, 9, 12345, dtype, 31, scale)
+    check_score(x, tok, token_logprobs(x, tok, top_k=11, temperature=T), T, 11)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -349,6 +360,21 @@ def test_score_gradient_masks_and_infinities(cuda):
     r = int(keep.nonzero()[0])
     p = torch.softmax(clean[r].double(), -1)
     assert (got[r].double() + p).abs().max() <= 200 * U
+
+
+def test_masked_rows_ignore_their_upstream_gradient(cuda):
+    """A masked row's gradient is 0 whatever comes back for it, NaN included."""
+    from macrogpt_jax_b200.distill import topk_distillation_loss
+    from macrogpt_jax_b200.logprobs import token_logprobs
+    x, tok, _ = make(cuda, 6, 4001, torch.bfloat16, 17)
+    keep = torch.tensor([1, 0, 1, 0, 0, 1], device=cuda).bool()
+    d = torch.where(keep, 1.0, float("nan"))
+    x = x.requires_grad_(True)
+    out = token_logprobs(x, tok, top_k=2, mask=keep)
+    loss = topk_distillation_loss(x, out.top_ids, out.top_logprobs.detach(), mask=keep)
+    for o, u in ((out.logprob, d), (out.entropy, d), (out.top_logprobs, d[:, None].expand(6, 2)), (loss, d)):
+        got, = torch.autograd.grad(o, x, u, retain_graph=True)
+        assert got[keep].isfinite().all() and got[keep].any() and (got[~keep] == 0).all()
 
 
 def test_score_gradient_by_differences(cuda):
