@@ -65,6 +65,8 @@ typedef struct CUstream_st* ufp8_stream_t; /* same handle as cudaStream_t */
 #define UFP8_K_MAJOR 0  /* stored [rows = M or N][K], K contiguous   */
 #define UFP8_MN_MAJOR 1 /* stored [K][cols = M or N], M/N contiguous */
 
+#define UFP8_LIKE_LOGITS (-1) /* gradient of logit rows in the logits' own type */
+
 /* output element type */
 #define UFP8_OUT_BF16 0
 #define UFP8_OUT_F32 1
@@ -317,14 +319,16 @@ int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens, int token
  * stride; 0: one value for all rows) and dtop (f32 [rows][top_k], with the forward's top_ids); NULL:
  * none.  dentropy needs a forward with `entropy`.  A masked row's gradient is 0.  Every column of every
  * row is written; fastest where an output row starts as far from a 16-byte boundary as its logit row.
- * For the logits of an output head (bf16 only): cap > 0 says that the logits are cap * tanh(l / cap) and
- * asks for the gradient at l (times 1 - (x / cap)^2; UFP8_EPI_XENT's soft cap), and *amax (NULL: not
- * wanted) becomes the largest |dlogits|, for ufp8_quantize. */
+ * fmt UFP8_LIKE_LOGITS: dlogits in the logits' type; amax and inv_scale unused, cap 0.
+ * fmt UFP8_E4M3 / UFP8_E5M2 (bf16 logits, an output head's): *amax = the largest |dlogits| that the rows'
+ * results allow (|dlogprob| + |dentropy| (1 / e + H) + sum |dtop|, over the temperature), s = FMAX / amax as
+ * ufp8_quantize derives it, dlogits = fp8(dl * s), *inv_scale = 1 / s; cap > 0 says that the logits are
+ * cap * tanh(l / cap) and asks for the gradient at l (times 1 - (x / cap)^2; UFP8_EPI_XENT's soft cap). */
 int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const void* tokens, int token_bytes,
                           const float* dlogprob, int64_t dlogprob_stride, const float* dentropy,
                           int64_t dentropy_stride, const float* dtop, const int64_t* top_ids, int64_t top_k,
-                          float cap, void* dlogits, int64_t out_stride_outer, int64_t out_stride_inner, float* amax,
-                          ufp8_stream_t stream);
+                          float cap, int fmt, void* dlogits, int64_t out_stride_outer, int64_t out_stride_inner,
+                          float* amax, float* inv_scale, ufp8_stream_t stream);
 
 /* Distillation from a teacher's top logits.  Per row, `entries` (0..1024) columns teacher_ids (int32 or
  * int64) with the teacher's logits or log probabilities there (UFP8_OUT_BF16 / UFP8_OUT_F32), both
@@ -337,11 +341,12 @@ int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const vo
 int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teacher_ids, int id_bytes, const void* teacher,
                          int teacher_dtype, int64_t entries, float* loss, float* stats, ufp8_stream_t stream);
 /* dlogits[v] = dloss / temperature * (p_v - sum of q_j with id_j == v), 0 for rows with loss 0 by the
- * rules above; arguments as in ufp8_logprob_backward.  The teacher gets no gradient. */
+ * rules above; arguments as in ufp8_logprob_backward (fp8: *amax = max |dloss| / temperature).  The teacher
+ * gets no gradient. */
 int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stats, const void* teacher_ids, int id_bytes,
                           const void* teacher, int teacher_dtype, int64_t entries, const float* dloss,
-                          int64_t dloss_stride, float cap, void* dlogits, int64_t out_stride_outer,
-                          int64_t out_stride_inner, float* amax, ufp8_stream_t stream);
+                          int64_t dloss_stride, float cap, int fmt, void* dlogits, int64_t out_stride_outer,
+                          int64_t out_stride_inner, float* amax, float* inv_scale, ufp8_stream_t stream);
 
 /* ---- Newton-Schulz orthogonalisation (Muon) ------------------------------------------------
  * Replaces orthogonalize (ueaj/opt/multiscale.py:110-141): optax.contrib's

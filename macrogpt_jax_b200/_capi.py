@@ -16,6 +16,7 @@ STATUS_WAIT_TIMEOUT, STATUS_PEER_TIMEOUT = 1, 2
 IPC_HANDLE_BYTES = 64
 AG_COPY_ENGINE, AG_SM = 0, 1
 E4M3, E5M2 = 0, 1
+LIKE_LOGITS = -1  # output format of the logit-row gradients: the logits' own type
 BF16 = 2  # bf16 GEMM operands; unquantised output of ufp8_xent_backward
 K_MAJOR, MN_MAJOR = 0, 1
 OUT_BF16, OUT_F32 = 0, 1
@@ -219,9 +220,10 @@ def load() -> ctypes.CDLL:
     lib.ufp8_xent_backward.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, vp, f32, i32, vp, i64, vp, vp, vp]
     rp = ctypes.POINTER(LogitRows)
     lib.ufp8_logprob_forward.argtypes = [rp, vp, i32, i64, vp, vp, vp, vp, vp, vp]
-    lib.ufp8_logprob_backward.argtypes = [rp, vp, vp, i32, vp, i64, vp, i64, vp, vp, i64, f32, vp, i64, i64, vp, vp]
+    lib.ufp8_logprob_backward.argtypes = [rp, vp, vp, i32, vp, i64, vp, i64, vp, vp, i64, f32, i32, vp, i64, i64, vp, vp,
+                                          vp]
     lib.ufp8_distill_forward.argtypes = [rp, vp, i32, vp, i32, i64, vp, vp, vp]
-    lib.ufp8_distill_backward.argtypes = [rp, vp, vp, i32, vp, i32, i64, vp, i64, f32, vp, i64, i64, vp, vp]
+    lib.ufp8_distill_backward.argtypes = [rp, vp, vp, i32, vp, i32, i64, vp, i64, f32, i32, vp, i64, i64, vp, vp, vp]
     lib.ufp8_newton_schulz_workspace.argtypes = [i64, i64, i64, ctypes.POINTER(i64)]
     lib.ufp8_newton_schulz.argtypes = [vp, i32, i64, i64, i64, i32, vp, f32, vp, i32, vp, i64, vp]
     lib.ufp8_rope_table.argtypes = [vp, i64, i64, vp, vp, vp, vp]
@@ -330,7 +332,7 @@ def xent_backward(logits_ptr, rows, V, ldl, labels_ptr, mask_ptr, lse_ptr, qrow_
 _entry = {}
 
 
-def _call(name: str, rows: LogitRows, args) -> None:
+def _call(name: str, rows: LogitRows, args, launches: int = 1) -> None:
     fn = _entry.get(name)
     if fn is None:
         fn = _entry[name] = getattr(load(), name)
@@ -338,7 +340,7 @@ def _call(name: str, rows: LogitRows, args) -> None:
     if rc:
         check(rc)
     if rows.rows > 0:
-        _count(1)
+        _count(launches)
 
 
 def logprob_forward(rows: LogitRows, *args) -> None:
@@ -347,8 +349,8 @@ def logprob_forward(rows: LogitRows, *args) -> None:
 
 
 def logprob_backward(rows: LogitRows, *args) -> None:
-    """ufp8_logprob_backward: the gradient of the above."""
-    _call("ufp8_logprob_backward", rows, args)
+    """ufp8_logprob_backward: the gradient of the above (fp8 output: its scale first)."""
+    _call("ufp8_logprob_backward", rows, args, 1 if args[11] == LIKE_LOGITS else 2)
 
 
 def distill_forward(rows: LogitRows, *args) -> None:
@@ -357,8 +359,8 @@ def distill_forward(rows: LogitRows, *args) -> None:
 
 
 def distill_backward(rows: LogitRows, *args) -> None:
-    """ufp8_distill_backward: the gradient of the above."""
-    _call("ufp8_distill_backward", rows, args)
+    """ufp8_distill_backward: the gradient of the above (fp8 output: its scale first)."""
+    _call("ufp8_distill_backward", rows, args, 1 if args[9] == LIKE_LOGITS else 2)
 
 
 def newton_schulz_workspace(batch: int, m: int, n: int) -> int:

@@ -22,7 +22,9 @@
 #include <cuda_bf16.h>
 
 #include <cmath>
+#include <type_traits>
 
+#include "fp8cast.cuh"
 #include "internal.h"
 
 namespace ufp8 {
@@ -1003,8 +1005,12 @@ struct GradArgs {
   int K;
   const float* dloss;
   int64_t dloss_stride;
-  float inv_cap;  // 1 / cap of logits that are cap * tanh(.), 0: not capped
-  uint32_t* amax;  // largest |output| as f32 bits (null: not wanted)
+  // fp8 output (an output head's logits): its format, 1 / cap of logits that are cap * tanh(.) (0: not
+  // capped), the bound of |output| and 1 / scale
+  int fmt;
+  float inv_cap;
+  float* amax;
+  float* inv_scale;
   void* out;
   int64_t out_outer, out_inner;  // row strides of the output
   int tasks;     // tasks of a row
@@ -1030,13 +1036,62 @@ __device__ __forceinline__ void load_entry(const GradArgs& a, int64_t row, int j
   }
 }
 
+// The largest |dlogits| that the rows' results allow, and the fp8 scale from it: |p - [label]|, |p - q| and the
+// derivative of the soft cap are at most 1, and p |log p + H| <= 1 / e + H.  fp8's exponent covers the factor by
+// which that is too large.  One CTA; a NaN is above all.
+template <bool kDistill>
+__global__ void __launch_bounds__(1024) rowamax_kernel(const GradArgs a) {
+  uint32_t top = 0;
+  for (int64_t r = threadIdx.x; r < a.r.rows; r += 1024) {
+    const float4 st = a.stats[r];
+    if ((a.r.mask && a.r.mask[r] == 0) || (kDistill && st.z == kNegInf)) continue;
+    float v;
+    if constexpr (kDistill) {
+      v = fabsf(a.dloss[r * a.dloss_stride]);
+    } else {
+      v = a.dlogprob ? fabsf(a.dlogprob[r * a.dlogprob_stride]) : 0.0f;
+      if (a.dentropy) v = __fmaf_rn(fabsf(a.dentropy[r * a.dentropy_stride]), __fadd_rn(0.368f, fabsf(st.z)), v);
+      if (a.dtop)
+        for (int j = 0; j < a.k; ++j) v = __fadd_rn(v, fabsf(a.dtop[r * a.k + j]));
+    }
+    top = max(top, __float_as_uint(__fmul_rn(v, a.r.inv_t)) & 0x7FFFFFFFu);
+  }
+  __shared__ uint32_t part[32];
+  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    top = __reduce_max_sync(0xFFFFFFFFu, part[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      const float amax = __uint_as_float(top);
+      *a.amax = amax;
+      *a.inv_scale = __fdiv_rn(1.0f, scale_from_amax(amax, a.fmt));
+    }
+  }
+}
+
+// Eight values of at most the format's largest (up to rounding) as fp8.  One finiteness test of their sum decides
+// whether the codes of NaN and infinities are needed.
+__device__ __forceinline__ uint2 to_fp8(const float (&v)[8], int fmt) {
+  const float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+  const __nv_fp8_interpretation_t kind = fmt == UFP8_E4M3 ? __NV_E4M3 : __NV_E5M2;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = isfinite(sum) ? static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]),
+                                                                          __NV_SATFINITE, kind))
+                         : cvt2(v[2 * i], v[2 * i + 1], fmt);
+  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+}
+
 // The warps of a resident grid walk (row, task) units on their own, without a barrier (with one step per CTA all
 // waited for the warp that sorted the entries in: 458 us at 4096 x 128256 with 64 of them, 340 so); a task is
 // `per_task` chunks of a row, a chunk 2 KB of it, kUnits 16-byte loads a lane.  Per task the warp works out the row
 // factors; per chunk it adds the weights of the row's entries that fall into it into `wt`, one f32 per
 // column and zero elsewhere, in entry order, so that the result does not depend on timing.  Then
 // v = p * factor + weight, and a lane with a weight in its columns sets those back to zero.
-// kHead: the logits are an output head's (soft cap, largest absolute value for the fp8 scale).
+// kHead: the logits are an output head's (bf16): the soft cap's derivative, and fp8 output by the scale of
+// rowamax_kernel.
 template <class T, bool kDistill, bool kHead>
 __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) {
   constexpr int kChunk = 32 * kUnits;  // units of a chunk
@@ -1051,7 +1106,7 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
   const int step_r = static_cast<int>(step / a.tasks), step_t = static_cast<int>(step % a.tasks);
   int row = static_cast<int>(first / a.tasks), task = static_cast<int>(first % a.tasks);
   const uint64_t c22 = pk(a.r.c2, a.r.c2), cap2 = pk(a.inv_cap, a.inv_cap);
-  float peak = 0.0f;
+  const float sc = kHead ? scale_from_amax(*a.amax, a.fmt) : 1.0f;
   const int n = kDistill ? a.K : (a.dlogprob ? 1 : 0) + (a.dtop ? a.k : 0);
   if (n > 0)
     for (int i = lane; i < kChunk * (kE / 4); i += 32) wt4[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1063,8 +1118,10 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
     }
     const RowIndex ri(a.r, row);
     const Row<T> x(a.r.x, ri.elem(a.r.stride_outer, a.r.stride_inner), a.r.V);
-    typename T::raw* o = static_cast<typename T::raw*>(a.out) + ri.elem(a.out_outer, a.out_inner);
-    const bool vec = ((reinterpret_cast<uintptr_t>(o) ^ reinterpret_cast<uintptr_t>(x.p)) & 15u) == 0;
+    using Out = std::conditional_t<kHead, uint8_t, typename T::raw>;
+    Out* o = static_cast<Out*>(a.out) + ri.elem(a.out_outer, a.out_inner);
+    // the units' first elements lie on multiples of a unit in the output, too
+    const bool vec = ((reinterpret_cast<uintptr_t>(o) - x.off * sizeof(Out)) & (kE * sizeof(Out) - 1)) == 0;
     const float4 st = a.stats[row];
     const bool dead = (a.r.mask && a.r.mask[row] == 0) || (kDistill && st.z == kNegInf);
     int u0 = task * a.per_task * kChunk;
@@ -1088,6 +1145,10 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
         }
         A = -__fmaf_rn(h, st.z, __fadd_rn(g, top));
         B = __fmul_rn(-h, kLn2);
+      }
+      if (kHead) {
+        A = __fmul_rn(A, sc);
+        B = __fmul_rn(B, sc);
       }
     }
     const uint64_t nm = pk(-st.x, -st.x), nl = pk(-st.y, -st.y);
@@ -1120,7 +1181,7 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
           const unsigned active = __ballot_sync(0xFFFFFFFFu, in);
           if (active == 0) continue;
           const float ew = kDistill ? __fmul_rn(-A, ex2a(__fmaf_rn(__fsub_rn(val, st.z), a.r.c2, -st.w)))
-                                    : __fmul_rn(val, a.r.inv_t);
+                                    : __fmul_rn(__fmul_rn(val, a.r.inv_t), sc);
           const int at = id - lo;
           for (unsigned left = active; left; left &= left - 1) {  // in entry order
             const int src = __ffs(left) - 1;
@@ -1168,42 +1229,44 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
               q[j / 4] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
           }
-          if (kHead) {
+          if (kHead && a.inv_cap > 0.0f) {
 #pragma unroll
             for (int j = 0; j < kE; j += 2) {
-              if (a.inv_cap > 0.0f) {  // times tanh' = 1 - (x / cap)^2
-                const uint64_t t = mul2(pk(v[j], v[j + 1]), cap2);
-                unpk(mul2(pk(g[j], g[j + 1]), fma2(t, neg2(t), pk(1.0f, 1.0f))), g[j], g[j + 1]);
-              }
-              peak = maxn(peak, maxn(fabsf(g[j]), fabsf(g[j + 1])));
+              const uint64_t t = mul2(pk(v[j], v[j + 1]), cap2);  // times tanh' = 1 - (x / cap)^2
+              unpk(mul2(pk(g[j], g[j + 1]), fma2(t, neg2(t), pk(1.0f, 1.0f))), g[j], g[j + 1]);
             }
           }
         }
         const int c = x.col(i);
+        // streaming stores: 4 % faster at 212 MB of gradient, 1 % at 1 GB
         if (whole || (vec && c >= 0 && c + kE <= x.V)) {
-          uint32_t q[4];
+          if constexpr (kHead) {
+            __stcs(reinterpret_cast<uint2*>(o + c), to_fp8(g, a.fmt));
+          } else {
+            uint32_t q[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (kE == 8) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(g[2 * j], g[2 * j + 1]);
-              q[j] = *reinterpret_cast<const uint32_t*>(&b);
-            } else {
-              q[j] = __float_as_uint(g[j]);
+            for (int j = 0; j < 4; ++j) {
+              if constexpr (kE == 8) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(g[2 * j], g[2 * j + 1]);
+                q[j] = *reinterpret_cast<const uint32_t*>(&b);
+              } else {
+                q[j] = __float_as_uint(g[j]);
+              }
             }
+            __stcs(reinterpret_cast<uint4*>(o + c), make_uint4(q[0], q[1], q[2], q[3]));
           }
-          // streaming stores: 4 % faster at 212 MB of gradient, 1 % at 1 GB
-          __stcs(reinterpret_cast<uint4*>(o + c), make_uint4(q[0], q[1], q[2], q[3]));
         } else {
 #pragma unroll
           for (int j = 0; j < kE; ++j)
-            if (c + j >= 0 && c + j < x.V) o[c + j] = T::from_f(g[j]);
+            if (c + j >= 0 && c + j < x.V) {
+              if constexpr (kHead)
+                o[c + j] = static_cast<uint8_t>(cvt2(g[j], 0.0f, a.fmt));
+              else
+                o[c + j] = T::from_f(g[j]);
+            }
         }
       }
     }
-  }
-  if (kHead && a.amax) {  // rounding is monotonic: the largest stored value is the largest one rounded
-    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(T::to_f(T::from_f(peak))) & 0x7FFFFFFFu);
-    if (lane == 0) atomicMax(a.amax, bits);
   }
 }
 
@@ -1345,27 +1408,33 @@ int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
 
 template <bool kDistill>
 int launch_grad(GradArgs& a, int dtype, const DeviceInfo& dev, cudaStream_t s) {
-  if (a.inv_cap > 0.0f || a.amax) {  // checked: bf16
-    if (a.amax) {
-      const cudaError_t e = cudaMemsetAsync(a.amax, 0, sizeof(float), s);
-      if (e != cudaSuccess) return cuda_error(e, "cudaMemsetAsync(amax)");
-    }
-    if (a.r.rows == 0) return UFP8_OK;
-    return launch_grad<Bf16, kDistill, true>(a, dev, s);
+  if (a.fmt != UFP8_LIKE_LOGITS) {  // checked: bf16
+    rowamax_kernel<kDistill><<<1, 1024, 0, s>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_error(e, "row amax launch");
+    return a.r.rows == 0 ? UFP8_OK : launch_grad<Bf16, kDistill, true>(a, dev, s);
   }
   return dtype == UFP8_OUT_F32 ? launch_grad<F32, kDistill, false>(a, dev, s)
                                : launch_grad<Bf16, kDistill, false>(a, dev, s);
 }
 
-// The output head's part of a backward: soft cap and amax, for bf16 logits.
-int head_args(const ufp8_logit_rows* x, float cap, float* amax, GradArgs* a, const char* who) {
+// The output head's part of a backward: soft cap and fp8 output, for bf16 logits.
+int head_args(const ufp8_logit_rows* x, float cap, int fmt, float* amax, float* inv_scale, GradArgs* a,
+              const char* who) {
+  const bool fp8 = fmt == UFP8_E4M3 || fmt == UFP8_E5M2;
+  if (!fp8 && fmt != UFP8_LIKE_LOGITS)
+    return set_error(UFP8_ERR_INVALID, "%s: fmt %d is not UFP8_E4M3/UFP8_E5M2/UFP8_LIKE_LOGITS", who, fmt);
   if (!(cap >= 0.0f) || std::isinf(cap))
     return set_error(UFP8_ERR_INVALID, "%s: cap must be 0 or a finite positive value", who);
-  if ((cap > 0.0f || amax) && x->dtype != UFP8_OUT_BF16)
-    return set_error(UFP8_ERR_UNSUPPORTED, "%s: cap and amax need bf16 logits", who);
-  if (!al(amax, 4)) return set_error(UFP8_ERR_ALIGN, "%s: amax not 4-byte aligned", who);
+  if (cap > 0.0f && !fp8) return set_error(UFP8_ERR_UNSUPPORTED, "%s: cap needs fp8 output", who);
+  if (fp8 && x->dtype != UFP8_OUT_BF16) return set_error(UFP8_ERR_UNSUPPORTED, "%s: fp8 output needs bf16 logits", who);
+  if (fp8 && (!amax || !inv_scale)) return set_error(UFP8_ERR_INVALID, "%s: null amax or inv_scale", who);
+  if (!al(amax, 4) || !al(inv_scale, 4))
+    return set_error(UFP8_ERR_ALIGN, "%s: amax or inv_scale not 4-byte aligned", who);
+  a->fmt = fmt;
   a->inv_cap = cap > 0.0f ? 1.0f / cap : 0.0f;
-  a->amax = reinterpret_cast<uint32_t*>(amax);
+  a->amax = amax;
+  a->inv_scale = inv_scale;
   return UFP8_OK;
 }
 
@@ -1410,21 +1479,21 @@ extern "C" int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens
 extern "C" int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const void* tokens,
                                      int token_bytes, const float* dlogprob, int64_t dlogprob_stride,
                                      const float* dentropy, int64_t dentropy_stride, const float* dtop,
-                                     const int64_t* top_ids, int64_t top_k, float cap, void* dlogits,
-                                     int64_t out_stride_outer, int64_t out_stride_inner, float* amax,
-                                     ufp8_stream_t stream) {
+                                     const int64_t* top_ids, int64_t top_k, float cap, int fmt,
+                                     void* dlogits, int64_t out_stride_outer, int64_t out_stride_inner, float* amax,
+                                     float* inv_scale, ufp8_stream_t stream) {
   const char* who = "ufp8_logprob_backward";
   GradArgs a{};
   if (int rc = rows_args(x, &a.r, who)) return rc;
   if (top_k < 0 || top_k > kMaxTop) return set_error(UFP8_ERR_INVALID, "%s: top_k must be 0..%d", who, kMaxTop);
   if (int rc = check_out(x, out_stride_outer, out_stride_inner, who)) return rc;
-  if (int rc = head_args(x, cap, amax, &a, who)) return rc;
+  if (int rc = head_args(x, cap, fmt, amax, inv_scale, &a, who)) return rc;
   if (dlogprob)
     if (int rc = check_ids(tokens, token_bytes, "tokens", who)) return rc;
   if (!al(stats, 16)) return set_error(UFP8_ERR_ALIGN, "%s: stats not 16-byte aligned", who);
-  if (!al(dlogits, x->dtype == UFP8_OUT_F32 ? 4 : 2))
+  if (fmt == UFP8_LIKE_LOGITS && !al(dlogits, x->dtype == UFP8_OUT_F32 ? 4 : 2))
     return set_error(UFP8_ERR_ALIGN, "%s: dlogits not aligned to their type", who);
-  if (x->rows == 0 && !amax) return UFP8_OK;
+  if (x->rows == 0 && fmt == UFP8_LIKE_LOGITS) return UFP8_OK;
   if (x->rows > 0 && (!stats || !dlogits)) return set_error(UFP8_ERR_INVALID, "%s: null stats or dlogits", who);
   if (x->rows > 0 && dlogprob && !tokens) return set_error(UFP8_ERR_INVALID, "%s: null tokens", who);
   if (dtop && (!top_ids || top_k == 0)) return set_error(UFP8_ERR_INVALID, "%s: null top_ids", who);
@@ -1488,19 +1557,19 @@ extern "C" int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teache
 
 extern "C" int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stats, const void* teacher_ids,
                                      int id_bytes, const void* teacher, int teacher_dtype, int64_t entries,
-                                     const float* dloss, int64_t dloss_stride, float cap, void* dlogits,
-                                     int64_t out_stride_outer, int64_t out_stride_inner, float* amax,
-                                     ufp8_stream_t stream) {
+                                     const float* dloss, int64_t dloss_stride, float cap, int fmt,
+                                     void* dlogits, int64_t out_stride_outer, int64_t out_stride_inner, float* amax,
+                                     float* inv_scale, ufp8_stream_t stream) {
   const char* who = "ufp8_distill_backward";
   GradArgs a{};
   if (int rc = rows_args(x, &a.r, who)) return rc;
   if (int rc = distill_check(x, teacher_ids, id_bytes, teacher, teacher_dtype, entries, who)) return rc;
   if (int rc = check_out(x, out_stride_outer, out_stride_inner, who)) return rc;
-  if (int rc = head_args(x, cap, amax, &a, who)) return rc;
+  if (int rc = head_args(x, cap, fmt, amax, inv_scale, &a, who)) return rc;
   if (!al(stats, 16)) return set_error(UFP8_ERR_ALIGN, "%s: stats not 16-byte aligned", who);
-  if (!al(dlogits, x->dtype == UFP8_OUT_F32 ? 4 : 2))
+  if (fmt == UFP8_LIKE_LOGITS && !al(dlogits, x->dtype == UFP8_OUT_F32 ? 4 : 2))
     return set_error(UFP8_ERR_ALIGN, "%s: dlogits not aligned to their type", who);
-  if (x->rows == 0 && !amax) return UFP8_OK;
+  if (x->rows == 0 && fmt == UFP8_LIKE_LOGITS) return UFP8_OK;
   if (x->rows > 0 && (!stats || !dlogits || !dloss))
     return set_error(UFP8_ERR_INVALID, "%s: null stats, dloss or dlogits", who);
   DeviceInfo* dev;

@@ -15,8 +15,8 @@ recomputed, which the reference's rematerialised chunks do (one GEMM of 2 T d V 
 
 `token_logprobs` and `distillation_loss` put the operators of logprobs.py and distill.py behind the
 same head (the teacher's targets, the scores of sampled tokens, the student's step): one node of the
-same kind, whose backward quantises the operator's bf16 logit gradient with the amax that the gradient
-kernel kept, and runs the two FP8 GEMMs and the norm's backward.
+same kind, whose backward writes the operator's logit gradient straight as fp8 (scale from the rows'
+results) and runs the two FP8 GEMMs and the norm's backward.
 """
 from __future__ import annotations
 
@@ -108,7 +108,7 @@ class _Score(NamedTuple):
 
     def backward(self, logits, stats, ids, grads, head):
         dlp, dent, dtop, _ = grads
-        ops.token_logprobs_backward(logits, stats, self.tokens, self.mask, self.temperature, dlp, dent, dtop,
+        return ops.token_logprobs_backward(logits, stats, self.tokens, self.mask, self.temperature, dlp, dent, dtop,
                                     ids[0] if ids else None, head)
 
 
@@ -126,7 +126,7 @@ class _Distill(NamedTuple):
         return (loss,), stats
 
     def backward(self, logits, stats, ids, grads, head):
-        ops.distill_backward(logits, stats, self.ids, self.teacher, self.mask, self.temperature, grads[0], head)
+        return ops.distill_backward(logits, stats, self.ids, self.teacher, self.mask, self.temperature, grads[0], head)
 
 
 @config

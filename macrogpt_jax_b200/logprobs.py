@@ -123,7 +123,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     `mask` [...] (bool or integer): a row whose mask is 0 is not read; it gives 0, 0, (-inf, -1) and a
     gradient of 0.  A logit of -inf has probability 0; a row of only -inf, or holding +inf or NaN, gives
     NaN.  Arithmetic is f32; gradients reach `logits` through logprob, entropy and top_logprobs, in the
-    logits' type."""
+    logits' type.  The same call gives the same bits; the last bits of a row may differ between calls
+    with other numbers of rows or another alignment, which group its sums differently."""
     who = "token_logprobs"
     check_logits(logits, who)
     lead, V = logits.shape[:-1], logits.shape[-1]

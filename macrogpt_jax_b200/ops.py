@@ -544,6 +544,12 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _dense(*tensors: torch.Tensor | None) -> None:
+    for t in tensors:
+        if t is not None and not t.is_contiguous():
+            raise ValueError("logit rows: tokens, ids, teacher values and masks must be contiguous")
+
+
 def _id_bytes(t: torch.Tensor | None) -> int:
     return 4 if t is not None and t.dtype == torch.int32 else 8
 
@@ -607,17 +613,21 @@ def _grad_rows(lr: LogitRows):
 
 
 def _grad_target(lr: LogitRows, head: tuple | None):
-    """(cap, dlogits, its row strides, amax) of a backward."""
+    """(cap, output format, dlogits, its row strides, amax, inv_scale) of a backward."""
     if head is None:
-        return (0.0, *_grad_rows(lr), None)
-    cap, out, amax_t = head
-    return cap, out, 0, out.stride(0), amax_t
+        return (0.0, C.LIKE_LOGITS, *_grad_rows(lr), None, None)
+    cap, fmt, pitch = head
+    dev = lr.logits.device
+    out = torch.empty((lr.rows, pitch), dtype=FP8_DTYPE[fmt], device=dev)
+    amax_t, inv = (torch.empty(1, dtype=torch.float32, device=dev) for _ in range(2))
+    return cap, fmt, out, 0, pitch, amax_t, inv
 
 
 def token_logprobs_forward(logits: torch.Tensor, tokens: torch.Tensor | None, mask: torch.Tensor | None, top_k: int,
                            temperature: float, entropy: bool, want_stats: bool):
     """(logprob, entropy, top log probabilities, top ids) over the logits' leading shape, then the
     backward's stats; None where not asked for (ufp8_logprob_forward)."""
+    _dense(tokens, mask)
     lr = logit_rows(logits)
     t, dev, f32 = lr.logits, logits.device, torch.float32
     lead = logits.shape[:-1]
@@ -646,25 +656,27 @@ def _row_grad(g: torch.Tensor | None):
 def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: torch.Tensor | None,
                             mask: torch.Tensor | None, temperature: float, dlp: torch.Tensor | None,
                             dent: torch.Tensor | None, dtop: torch.Tensor | None, top_id: torch.Tensor | None,
-                            head: tuple | None = None) -> torch.Tensor:
-    """dlogits of token_logprobs_forward (ufp8_logprob_backward).  `head`: (soft cap, dlogits buffer
-    [rows, pitch], amax) of an output head, see head_rows_backward."""
+                            head: tuple | None = None) -> torch.Tensor | Fp8Tensor:
+    """dlogits of token_logprobs_forward (ufp8_logprob_backward).  `head`: (soft cap, fp8 format, pitch) of
+    an output head: an Fp8Tensor [rows, pitch] of the gradient before the cap."""
+    _dense(tokens, mask, top_id)
     lr = logit_rows(logits)
     t = lr.logits
     dlp, s_lp = _row_grad(dlp)
     dent, s_ent = _row_grad(dent)
     dtop = None if dtop is None else dtop.to(torch.float32).contiguous()
     top_k = top_id.shape[-1] if dtop is not None else 0
-    cap, out, outer, inner, amax_t = _grad_target(lr, head)
+    cap, fmt, out, outer, inner, amax_t, inv = _grad_target(lr, head)
     _call_on(t, "logprob_grad", 2.0, C.logprob_backward, lr.c(temperature, mask), stats.data_ptr(), _ptr(tokens),
              _id_bytes(tokens), _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, cap,
-             out.data_ptr(), outer, inner, _ptr(amax_t))
-    return out
+             fmt, out.data_ptr(), outer, inner, _ptr(amax_t), _ptr(inv))
+    return out if head is None else Fp8Tensor(out, inv, amax_t)
 
 
 def distill_forward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, mask: torch.Tensor | None,
                     temperature: float, want_stats: bool):
     """(loss over the logits' leading shape, the backward's stats) (ufp8_distill_forward)."""
+    _dense(ids, teacher, mask)
     lr = logit_rows(logits)
     t = lr.logits
     loss = _empty_f32(logits.shape[:-1], t.device)
@@ -676,21 +688,22 @@ def distill_forward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tens
 
 def distill_backward(logits: torch.Tensor, stats: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
                      mask: torch.Tensor | None, temperature: float, dloss: torch.Tensor,
-                     head: tuple | None = None) -> torch.Tensor:
+                     head: tuple | None = None) -> torch.Tensor | Fp8Tensor:
     """dlogits of distill_forward (ufp8_distill_backward); `head` as in token_logprobs_backward."""
+    _dense(ids, teacher, mask)
     lr = logit_rows(logits)
     t = lr.logits
     dloss, stride = _row_grad(dloss)
-    cap, out, outer, inner, amax_t = _grad_target(lr, head)
+    cap, fmt, out, outer, inner, amax_t, inv = _grad_target(lr, head)
     _call_on(t, "distill_grad", 2.0, C.distill_backward, lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(),
              _id_bytes(ids), teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride,
-             cap, out.data_ptr(), outer, inner, _ptr(amax_t))
-    return out
+             cap, fmt, out.data_ptr(), outer, inner, _ptr(amax_t), _ptr(inv))
+    return out if head is None else Fp8Tensor(out, inv, amax_t)
 
 
 # The same operators behind the fused output head: final norm -> FP8 lm_head (soft cap in its epilogue) ->
-# logits [T, Vp] -> operator, whose dlogits (bf16, with their amax from the same kernel) are quantised for
-# the two backward GEMMs.
+# logits [T, Vp] -> operator, whose gradient kernel writes fp8 dlogits for the two backward GEMMs (scale
+# from the rows' results, no pass over the gradient for its amax).
 def head_rows_forward(x2d: torch.Tensor, scale: torch.Tensor | None, centered: bool, eps: float, w: torch.Tensor,
                       cap: float):
     """(logits bf16 [T, Vp] of which columns < V count, saved)."""
@@ -703,14 +716,11 @@ def head_rows_forward(x2d: torch.Tensor, scale: torch.Tensor | None, centered: b
 
 def head_rows_backward(grad_fn, logits: torch.Tensor, saved, V: int, cap: float, need_dw: bool, fmt: int):
     """Backward of head_rows_forward up to the norm: (dxn bf16 [T, d], dw bf16 [d, V] or None).
-    grad_fn(logits [T, V], head) writes dlogits as token_logprobs_backward and distill_backward do."""
+    grad_fn(logits [T, V], head) gives dlogits as token_logprobs_backward and distill_backward do."""
     qx, _, qw = saved
     T, d = qx.q.shape
-    dl = torch.empty_like(logits)
-    amax_t = torch.empty(1, dtype=torch.float32, device=logits.device)
-    grad_fn(logits[:, :V], (cap, dl, amax_t))
-    qd = quantize(dl, fmt, amax_t)
     Vp = logits.shape[1]
+    qd = grad_fn(logits[:, :V], (cap, fmt, Vp))
     dxn = torch.empty((T, d), dtype=torch.bfloat16, device=logits.device)
     gemm(operand(qd, C.K_MAJOR, Vp), operand(qw, C.K_MAJOR, Vp), T, d, V, dxn, d)
     dw = None

@@ -4,9 +4,10 @@ fp8 recipe, and its gradients against a plain computation of the same recipe.
 
 Tolerances.  The node's logits and the plain ones are one bf16 rounding of two f32 sums in different
 orders (and a soft cap of three roundings): at most one bf16 step apart, which is 2^-4 for 8 <= |logit| <
-16.  A log probability moves by at most |dx_t| + sum_v p_v |dx_v|, so by two steps: 2^-3.  Gradients go through fp8 GEMMs: the tolerance of helpers.py against a reference
-that quantises the same way.  The logit gradient is checked before the fp8 cast, on the kernels
-themselves: half a bf16 step and the f32 terms of test_gpu_logprob.py."""
+16.  A log probability moves by at most |dx_t| + sum_v p_v |dx_v|, so by two steps: 2^-3.  Gradients go
+through fp8 GEMMs: the tolerance of helpers.py against a reference that quantises the same way, with the
+same scale (from the bound of |dl| that the rows' results allow).  The fp8 logit gradient itself is checked
+on the kernels: half a step of the format."""
 import pytest
 import torch
 
@@ -28,8 +29,8 @@ def make_head(cuda, d, V, cap, seed=0):
     return head, x, g
 
 
-def fp8(t, dt, fmax):
-    s = fmax / t.abs().max().float().clamp(min=1e-30)
+def fp8(t, dt, fmax, amax=None):
+    s = fmax / (t.abs().max().float().clamp(min=1e-30) if amax is None else amax)
     return (t.float() * s).to(dt).float() / s
 
 
@@ -51,9 +52,9 @@ def plain_logits(head, x):
     return capped(head, *plain_operands(head, xn))
 
 
-def head_reference(head, x, grad_logits):
+def head_reference(head, x, grad_logits, bound):
     """Gradients of sum(<grad_logits(logits), logits>) with the node's recipe: e4m3 operands, the logit
-    gradient in the lm_head's bwd_dtype, both per tensor, f32 products, the norm by autograd."""
+    gradient in the lm_head's bwd_dtype with the scale of `bound`, f32 products, the norm by autograd."""
     x = x.detach().float().requires_grad_(True)
     scale = head.norm.scale.detach().float().requires_grad_(True)
     xn = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + head.norm.eps) * scale
@@ -62,7 +63,7 @@ def head_reference(head, x, grad_logits):
     dl = grad_logits(c)
     if head.head_cap == "tanh":
         dl = dl * (1 - (c / 15) ** 2)
-    qd = fp8(dl.bfloat16(), torch.float8_e5m2, 57344.0)
+    qd = fp8(dl, torch.float8_e5m2, 57344.0, bound)
     dw = qx.reshape(-1, qx.shape[-1]).T @ qd.reshape(-1, qd.shape[-1])
     dxn = (qd @ qw.T).bfloat16().float()
     dx, ds = torch.autograd.grad(xn, (x, scale), dxn)
@@ -111,7 +112,8 @@ def test_head_score_gradients(cuda, cap, V):
         val = val + (lp.gather(2, out.top_ids.clamp(min=0)) * dtop)[mask].sum()
         return torch.autograd.grad(val, c)[0].float()
 
-    dx, ds, dw = head_reference(head, x, grad)
+    bound = ((adv.abs() + 0.05 * (0.368 + out.entropy.detach()) + dtop.abs().sum(-1)) * mask).max()
+    dx, ds, dw = head_reference(head, x, grad, bound)
     for a, b in ((x.grad, dx), (head.norm.scale.grad, ds), (head.lm_head.w.grad, dw)):
         compare(a.double().cpu().numpy(), b.double().cpu().numpy())
 
@@ -146,14 +148,16 @@ def test_teacher_head_to_student_head(cuda, cap, V, T):
         c = c.double().requires_grad_(True)
         return torch.autograd.grad(value(c).sum(), c)[0].float()
 
-    dx, ds, dw = head_reference(student, x, grad)
+    dx, ds, dw = head_reference(student, x, grad, torch.tensor(1 / T, device=cuda))
     for a, b in ((x.grad, dx), (student.norm.scale.grad, ds), (student.lm_head.w.grad, dw)):
         compare(a.double().cpu().numpy(), b.double().cpu().numpy())
 
 
-def test_head_gradient_kernel(cuda):
-    """Soft cap, amax and a padded pitch in the gradient kernel: dlogits against the formula, amax the
-    largest stored value, 0 where every row is masked."""
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("cap", [0.0, 15.0])
+def test_head_gradient_kernel(cuda, fmt, cap):
+    """The gradient kernel's fp8 output (soft cap, padded pitch): dlogits against the formula, the scale from
+    the rows' bound, zeros where every row is masked."""
     from macrogpt_jax_b200 import ops
     T, V, Vp = 37, 1000, 1008
     g = torch.Generator(device=cuda).manual_seed(7)
@@ -162,24 +166,43 @@ def test_head_gradient_kernel(cuda):
     mask = torch.rand(T, generator=g, device=cuda) > 0.5
     adv = torch.randn(T, generator=g, device=cuda)
     lg = c[:, :V]
-    stats = ops.token_logprobs_forward(lg, tok, mask, 0, 1.0, True, True)[4]
-    out = torch.full((T, Vp), 7.0, dtype=torch.bfloat16, device=cuda)
-    amax = torch.empty(1, device=cuda)
-    ops.token_logprobs_backward(lg, stats, tok, mask, 1.0, adv, None, None, None, (15.0, out, amax))
-    x = lg.double()
-    p = torch.softmax(x, -1)
-    cap = 1 - (x / 15) ** 2
-    one = torch.zeros_like(p).scatter_(1, tok[:, None], 1.0)
-    ref = (one - p) * adv.double()[:, None] * cap * mask[:, None]
-    # f32: p to 100 u, cap's two roundings relative to 1, the factor's three
-    tol = 2.0 ** -24 * adv.double().abs()[:, None] * (100 * p + 8 * one + 8 * (one - p).abs())
-    half = torch.finfo(torch.bfloat16).eps / 2
-    assert ((out[:, :V].double() - ref).abs() <= tol + half * ref.abs()).all()
-    assert (out[:, V:] == 7.0).all()
-    assert amax.item() == out[:, :V].abs().max().item()
+    out = ops.token_logprobs_forward(lg, tok, mask, 4, 1.0, True, True)
+    ent, top_id, stats = out[1], out[3], out[4]
+    dent = torch.full((T,), 0.1, device=cuda)
+    dtop = torch.randn((T, 4), generator=g, device=cuda) * 0.1
+    q = ops.token_logprobs_backward(lg, stats, tok, mask, 1.0, adv, dent, dtop, top_id, (cap, fmt, Vp))
+    assert q.q.shape == (T, Vp)
+    fmax, eps, tiny = ((448.0, 2.0 ** -3, 2.0 ** -9), (57344.0, 2.0 ** -2, 2.0 ** -16))[fmt]
+    # the bound, and inv_scale = 1 / (fmax / amax): three roundings
+    bound = ((adv.abs() + 0.1 * (0.368 + ent.abs()) + dtop.abs().sum(1)) * mask).double().max()
+    assert abs(q.amax.item() - bound) <= 8 * 2.0 ** -24 * bound
+    assert abs(q.inv_scale.item() - q.amax.item() / fmax) <= 3 * 2.0 ** -24 * q.amax.item() / fmax
+    x = lg.double().requires_grad_(True)
+    lp = torch.log_softmax(x, -1)
+    val = lp.gather(1, tok[:, None])[:, 0] * adv + 0.1 * -(lp.exp() * lp).sum(-1)
+    val = (val + (lp.gather(1, top_id.clamp(min=0)) * dtop).sum(-1))[mask].sum()
+    ref, = torch.autograd.grad(val, x)
+    ref = ref * (1 - (x.detach() / cap) ** 2) if cap else ref
+    deq = q.q[:, :V].double() * q.inv_scale.double()
+    # half a step of the format (relative, or of its subnormals), and f32 work on values below `bound`
+    tol = eps / 2 * ref.abs() + tiny / 2 * q.inv_scale.double() + 200 * 2.0 ** -24 * bound
+    assert ((deq - ref).abs() <= tol).all(), ((deq - ref).abs() / tol).max()
+    assert ref.abs().max() <= bound
     none = torch.zeros(T, dtype=torch.bool, device=cuda)
-    ops.token_logprobs_backward(lg, stats, tok, none, 1.0, adv, None, None, None, (15.0, out, amax))
-    assert amax.item() == 0 and not out[:, :V].any()
+    q = ops.token_logprobs_backward(lg, stats, tok, none, 1.0, adv, None, None, None, (cap, fmt, Vp))
+    assert q.amax.item() == 0 and q.inv_scale.item() == 1 and not q.q[:, :V].view(torch.uint8).any()
+    # distillation: the bound is the largest upstream gradient
+    ids = torch.rand((T, V), generator=g, device=cuda).argsort(-1)[:, :9].contiguous()
+    t = torch.randn((T, 9), generator=g, device=cuda)
+    dstats = ops.distill_forward(lg, ids, t, mask, 2.0, True)[1]
+    q = ops.distill_backward(lg, dstats, ids, t, mask, 2.0, adv, (cap, fmt, Vp))
+    assert q.amax.item() == (adv.abs() * mask).max().item() * 0.5
+    dense = torch.zeros((T, V), dtype=torch.float64, device=cuda).scatter_(1, ids, torch.softmax(t.double() / 2, -1))
+    ref = (torch.softmax(lg.double() / 2, -1) - dense) * (adv.double() * mask / 2)[:, None]
+    ref = ref * (1 - (lg.double() / cap) ** 2) if cap else ref
+    deq = q.q[:, :V].double() * q.inv_scale.double()
+    tol = eps / 2 * ref.abs() + tiny / 2 * q.inv_scale.double() + 200 * 2.0 ** -24 * q.amax.double()
+    assert ((deq - ref).abs() <= tol).all()
 
 
 def test_head_retained_graph_and_changed_inputs(cuda):

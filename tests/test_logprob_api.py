@@ -27,20 +27,20 @@ def fwd(r, tokens=P, token_bytes=8, k=0, lp=P, ent=P, top=None, ids=None, stats=
                                          ids, stats, None)
 
 
-def bwd(r, stats=P, tokens=P, token_bytes=8, dlp=P, dtop=None, ids=None, k=0, cap=0.0, out=P, outer=400, inner=100,
-        amax=None):
+def bwd(r, stats=P, tokens=P, token_bytes=8, dlp=P, dtop=None, ids=None, k=0, cap=0.0, fmt=C.LIKE_LOGITS, out=P,
+        outer=400, inner=100, amax=None, inv=None):
     return C.load().ufp8_logprob_backward(ctypes.byref(r), stats, tokens, token_bytes, dlp, 1, None, 0, dtop, ids, k,
-                                          cap, out, outer, inner, amax, None)
+                                          cap, fmt, out, outer, inner, amax, inv, None)
 
 
 def dfwd(r, ids=P, id_bytes=8, teacher=P, dtype=C.OUT_F32, k=4, loss=P, stats=None):
     return C.load().ufp8_distill_forward(ctypes.byref(r), ids, id_bytes, teacher, dtype, k, loss, stats, None)
 
 
-def dbwd(r, stats=P, ids=P, id_bytes=8, teacher=P, dtype=C.OUT_F32, k=4, dloss=P, cap=0.0, out=P, outer=400,
-         inner=100, amax=None):
+def dbwd(r, stats=P, ids=P, id_bytes=8, teacher=P, dtype=C.OUT_F32, k=4, dloss=P, cap=0.0, fmt=C.LIKE_LOGITS,
+         out=P, outer=400, inner=100, amax=None, inv=None):
     return C.load().ufp8_distill_backward(ctypes.byref(r), stats, ids, id_bytes, teacher, dtype, k, dloss, 1, cap,
-                                          out, outer, inner, amax, None)
+                                          fmt, out, outer, inner, amax, inv, None)
 
 
 @pytest.mark.parametrize("call,code,msg", [
@@ -77,10 +77,14 @@ def dbwd(r, stats=P, ids=P, id_bytes=8, teacher=P, dtype=C.OUT_F32, k=4, dloss=P
     (lambda: bwd(rows(), dtop=P, ids=P, k=0), C.ERR_INVALID, "null top_ids"),
     (lambda: bwd(rows(), cap=-1.0), C.ERR_INVALID, "cap must be"),
     (lambda: bwd(rows(), cap=float("inf")), C.ERR_INVALID, "cap must be"),
-    (lambda: bwd(rows(dtype=C.OUT_F32), cap=15.0), C.ERR_UNSUPPORTED, "bf16"),
-    (lambda: bwd(rows(), amax=P + 2), C.ERR_ALIGN, "amax"),
-    (lambda: dbwd(rows(dtype=C.OUT_F32), amax=P), C.ERR_UNSUPPORTED, "bf16"),
     (lambda: dbwd(rows(), cap=float("nan")), C.ERR_INVALID, "cap must be"),
+    (lambda: bwd(rows(), cap=15.0), C.ERR_UNSUPPORTED, "cap needs fp8"),
+    (lambda: bwd(rows(), fmt=C.BF16), C.ERR_INVALID, "fmt 2"),
+    (lambda: bwd(rows(dtype=C.OUT_F32), fmt=C.E5M2, amax=P, inv=P), C.ERR_UNSUPPORTED, "bf16"),
+    (lambda: dbwd(rows(dtype=C.OUT_F32), fmt=C.E4M3, amax=P, inv=P), C.ERR_UNSUPPORTED, "bf16"),
+    (lambda: bwd(rows(), fmt=C.E5M2), C.ERR_INVALID, "null amax"),
+    (lambda: dbwd(rows(), fmt=C.E5M2, amax=P), C.ERR_INVALID, "null amax or inv_scale"),
+    (lambda: bwd(rows(), fmt=C.E5M2, amax=P + 2, inv=P), C.ERR_ALIGN, "amax"),
     (lambda: dfwd(rows(), k=-1), C.ERR_INVALID, "entries must be"),
     (lambda: dfwd(rows(), k=1025), C.ERR_INVALID, "entries must be"),
     (lambda: dfwd(rows(), dtype=9), C.ERR_INVALID, "teacher_dtype 9"),
