@@ -176,6 +176,11 @@ class OutputHead(torch.nn.Module):
                                  ops.FMT_OF_DTYPE[self.lm_head.bwd_dtype])
         return loss.reshape(lead)
 
+    def _check_width(self, activations: torch.Tensor, who: str) -> None:
+        """Another width flattens to another number of rows than the tokens, ids and masks have."""
+        if activations.shape[-1:] != (self.model_d,):
+            raise ValueError(f"{who}: activations {tuple(activations.shape)}, expected [..., {self.model_d}]")
+
     def _rows(self, activations: torch.Tensor, op):
         """op's outputs on the logits of the flattened activations, through the fused node."""
         x2d = activations.to(torch.bfloat16).reshape(-1, self.model_d).contiguous()
@@ -193,10 +198,11 @@ class OutputHead(torch.nn.Module):
                        entropy: bool = True) -> TokenLogprobs:
         """logprobs.token_logprobs(self.get_logits(activations), ...), through the fused node when
         fused() holds (then the gradients reach the activations, the norm and the lm_head)."""
+        who, lead = "OutputHead.token_logprobs", activations.shape[:-1]
+        self._check_width(activations, who)
         if not self.fused():
             return token_logprobs(self.get_logits(activations), tokens, top_k=top_k, temperature=temperature, mask=mask,
                                   entropy=entropy)
-        who, lead = "OutputHead.token_logprobs", activations.shape[:-1]
         check_logits(activations, who)
         temperature = check_score(tokens, top_k, self.vocab_size, temperature, entropy, who)
         if tokens is not None:
@@ -212,10 +218,11 @@ class OutputHead(torch.nn.Module):
                           temperature: float = 1.0, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """distill.topk_distillation_loss(self.get_logits(activations), ...), through the fused node when
         fused() holds."""
+        who, lead = "OutputHead.distillation_loss", activations.shape[:-1]
+        self._check_width(activations, who)
         if not self.fused():
             return topk_distillation_loss(self.get_logits(activations), teacher_ids, teacher_logits,
                                           temperature=temperature, mask=mask)
-        who, lead = "OutputHead.distillation_loss", activations.shape[:-1]
         check_logits(activations, who)
         temperature = check_temperature(temperature, who)
         ids, teacher = check_teacher(teacher_ids, teacher_logits, activations, who)

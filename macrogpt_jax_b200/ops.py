@@ -537,21 +537,33 @@ class LogitRows(NamedTuple):
     def c(self, temperature: float, mask: torch.Tensor | None) -> C.LogitRows:
         t = self.logits
         return C.LogitRows(t.data_ptr(), _LOGIT_DTYPE[t.dtype], temperature, self.rows, t.shape[-1], self.inner,
-                           self.stride_outer, self.stride_inner, _ptr(mask))
+                           self.stride_outer, self.stride_inner, _mask_ptr(mask))
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _dense(*tensors: torch.Tensor | None) -> None:
+def _dense(rows: int, *tensors: torch.Tensor | None, per_row: int = 1) -> None:
+    """The kernels index these by row: a tensor of another size would be read or written past its end."""
     for t in tensors:
-        if t is not None and not t.is_contiguous():
-            raise ValueError("logit rows: tokens, ids, teacher values and masks must be contiguous")
+        if t is not None and (t.numel() != rows * per_row or not t.is_contiguous()):
+            raise ValueError(f"logit rows: a tensor {tuple(t.shape)} with strides {t.stride()} where {rows} rows of "
+                             f"{per_row} values, contiguous, belong")
 
 
 def _id_bytes(t: torch.Tensor | None) -> int:
-    return 4 if t is not None and t.dtype == torch.int32 else 8
+    if t is None or t.dtype == torch.int64:
+        return 8
+    if t.dtype != torch.int32:
+        raise TypeError(f"logit rows: tokens and ids are int32 or int64, got {t.dtype}")
+    return 4
+
+
+def _mask_ptr(mask: torch.Tensor | None) -> int | None:
+    if mask is not None and mask.element_size() != 1:
+        raise TypeError(f"logit rows: the mask is one byte per row, got {mask.dtype}")
+    return _ptr(mask)
 
 
 def _empty_f32(shape, device) -> torch.Tensor:
@@ -627,8 +639,8 @@ def token_logprobs_forward(logits: torch.Tensor, tokens: torch.Tensor | None, ma
                            temperature: float, entropy: bool, want_stats: bool):
     """(logprob, entropy, top log probabilities, top ids) over the logits' leading shape, then the
     backward's stats; None where not asked for (ufp8_logprob_forward)."""
-    _dense(tokens, mask)
     lr = logit_rows(logits)
+    _dense(lr.rows, tokens, mask)
     t, dev, f32 = lr.logits, logits.device, torch.float32
     lead = logits.shape[:-1]
     lp = torch.empty_like(tokens, dtype=f32) if tokens is not None else None
@@ -641,11 +653,13 @@ def token_logprobs_forward(logits: torch.Tensor, tokens: torch.Tensor | None, ma
     return lp, ent, top_lp, top_id, stats
 
 
-def _row_grad(g: torch.Tensor | None):
+def _row_grad(g: torch.Tensor | None, rows: int):
     """An upstream gradient of one f32 per row as (tensor, elements between rows): 0 for one value
     expanded over the rows (what .sum() and .mean() send back)."""
     if g is None:
         return None, 0
+    if g.numel() != rows:
+        raise ValueError(f"logit rows: an upstream gradient {tuple(g.shape)} for {rows} rows")
     if g.dtype != torch.float32:
         g = g.to(torch.float32)
     if g.is_contiguous():
@@ -659,13 +673,16 @@ def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: t
                             head: tuple | None = None) -> torch.Tensor | Fp8Tensor:
     """dlogits of token_logprobs_forward (ufp8_logprob_backward).  `head`: (soft cap, fp8 format, pitch) of
     an output head: an Fp8Tensor [rows, pitch] of the gradient before the cap."""
-    _dense(tokens, mask, top_id)
     lr = logit_rows(logits)
     t = lr.logits
-    dlp, s_lp = _row_grad(dlp)
-    dent, s_ent = _row_grad(dent)
+    dlp, s_lp = _row_grad(dlp, lr.rows)
+    dent, s_ent = _row_grad(dent, lr.rows)
     dtop = None if dtop is None else dtop.to(torch.float32).contiguous()
     top_k = top_id.shape[-1] if dtop is not None else 0
+    _dense(lr.rows, tokens, mask)
+    _dense(lr.rows, stats, per_row=4)
+    if dtop is not None:
+        _dense(lr.rows, dtop, top_id, per_row=top_k)
     cap, fmt, out, outer, inner, amax_t, inv = _grad_target(lr, head)
     _call_on(t, "logprob_grad", 2.0, C.logprob_backward, lr.c(temperature, mask), stats.data_ptr(), _ptr(tokens),
              _id_bytes(tokens), _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, cap,
@@ -676,8 +693,9 @@ def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: t
 def distill_forward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, mask: torch.Tensor | None,
                     temperature: float, want_stats: bool):
     """(loss over the logits' leading shape, the backward's stats) (ufp8_distill_forward)."""
-    _dense(ids, teacher, mask)
     lr = logit_rows(logits)
+    _dense(lr.rows, mask)
+    _dense(lr.rows, ids, teacher, per_row=ids.shape[-1])
     t = lr.logits
     loss = _empty_f32(logits.shape[:-1], t.device)
     stats = torch.empty(lr.rows, 4, dtype=torch.float32, device=t.device) if want_stats else None
@@ -690,10 +708,12 @@ def distill_backward(logits: torch.Tensor, stats: torch.Tensor, ids: torch.Tenso
                      mask: torch.Tensor | None, temperature: float, dloss: torch.Tensor,
                      head: tuple | None = None) -> torch.Tensor | Fp8Tensor:
     """dlogits of distill_forward (ufp8_distill_backward); `head` as in token_logprobs_backward."""
-    _dense(ids, teacher, mask)
     lr = logit_rows(logits)
+    _dense(lr.rows, mask)
+    _dense(lr.rows, ids, teacher, per_row=ids.shape[-1])
+    _dense(lr.rows, stats, per_row=4)
     t = lr.logits
-    dloss, stride = _row_grad(dloss)
+    dloss, stride = _row_grad(dloss, lr.rows)
     cap, fmt, out, outer, inner, amax_t, inv = _grad_target(lr, head)
     _call_on(t, "distill_grad", 2.0, C.distill_backward, lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(),
              _id_bytes(ids), teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride,

@@ -1,0 +1,103 @@
+"""Refusals of OutputHead.token_logprobs / distillation_loss and of the logit-row functions below them,
+without a GPU: nothing may reach a kernel with fewer values than it has rows.  Tensors are fake ones on a
+CUDA device (shapes and types, no data) or CPU tensors that no check here lets through to a launch."""
+import pytest
+import torch
+from torch._subclasses import FakeTensorMode
+
+from macrogpt_jax_b200 import _capi as C
+from macrogpt_jax_b200 import ops
+
+D, V = 16, 40
+
+
+@pytest.fixture(params=["fused", "generic"])
+def head(request):
+    from macrogpt_jax_b200.einsum import Rngs
+    from macrogpt_jax_b200.head import OutputHead
+    h = OutputHead(D, V, rngs=Rngs(0))
+    if request.param == "generic":
+        h.norm.scale.data = h.norm.scale.data.float()
+    assert h.fused() == (request.param == "fused")
+    return h
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The logit-row entry points of the library replaced by a record of their rows."""
+    calls = []
+    for name in ("logprob_forward", "logprob_backward", "distill_forward", "distill_backward"):
+        monkeypatch.setattr(C, name, lambda rows, *args, name=name: calls.append((name, rows.rows)))
+    monkeypatch.setattr(ops, "_call_on", lambda t, kind, passes, fn, *args: fn(*args, None))
+    return calls
+
+
+def fake(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="cuda")
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 2 * D), (2, 3, D // 2), (2, 3, D + 1), (2, D, 3), ()])
+def test_head_refuses_activations_of_another_width(head, shape):
+    lead = shape[:-1]
+    with FakeTensorMode():
+        x = fake(*shape)
+        tok = fake(*lead, dtype=torch.int64)
+        with pytest.raises(ValueError, match="token_logprobs: activations"):
+            head.token_logprobs(x, tok)
+        with pytest.raises(ValueError, match="distillation_loss: activations"):
+            head.distillation_loss(x, fake(*lead, 4, dtype=torch.int64), fake(*lead, 4))
+
+
+ROWS = 12
+
+
+def args(n=ROWS, k=3):
+    """(logits of ROWS rows, tokens, mask, ids, teacher, stats, upstream, dtop) for n rows."""
+    return (torch.zeros(ROWS, V), torch.zeros(n, dtype=torch.int64), torch.ones(n, dtype=torch.bool),
+            torch.zeros(n, k, dtype=torch.int64), torch.zeros(n, k), torch.zeros(n, 4), torch.zeros(n),
+            torch.zeros(n, k))
+
+
+def test_functions_take_matching_rows(launches):
+    x, tok, mask, ids, teacher, stats, up, dtop = args()
+    ops.token_logprobs_forward(x, tok, mask, 3, 1.0, True, True)
+    ops.token_logprobs_backward(x, stats, tok, mask, 1.0, up, up, dtop, ids)
+    ops.distill_forward(x, ids, teacher, mask, 1.0, True)
+    ops.distill_backward(x, stats, ids, teacher, mask, 1.0, up.sum().expand(ROWS))
+    assert launches == [(n, ROWS) for n in ("logprob_forward", "logprob_backward", "distill_forward",
+                                            "distill_backward")]
+
+
+@pytest.mark.parametrize("n", [6, 11, 13, 24])
+@pytest.mark.parametrize("which", range(12))
+def test_functions_refuse_other_numbers_of_rows(launches, n, which):
+    x, tok, mask, ids, teacher, stats, up, dtop = args()
+    _, tok2, mask2, ids2, teacher2, stats2, up2, dtop2 = args(n)
+    bad = [lambda: ops.token_logprobs_forward(x, tok2, None, 0, 1.0, True, True),
+           lambda: ops.token_logprobs_forward(x, tok, mask2, 0, 1.0, True, True),
+           lambda: ops.token_logprobs_backward(x, stats, tok2, None, 1.0, up, None, None, None),
+           lambda: ops.token_logprobs_backward(x, stats, tok, mask2, 1.0, up, None, None, None),
+           lambda: ops.token_logprobs_backward(x, stats2, tok, None, 1.0, up, None, None, None),
+           lambda: ops.token_logprobs_backward(x, stats, tok, None, 1.0, up2, None, None, None),
+           lambda: ops.token_logprobs_backward(x, stats, tok, None, 1.0, None, up2, None, None),
+           lambda: ops.token_logprobs_backward(x, stats, tok, None, 1.0, None, None, dtop2, ids),
+           lambda: ops.distill_forward(x, ids2, teacher2, None, 1.0, True),
+           lambda: ops.distill_forward(x, ids, teacher, mask2, 1.0, True),
+           lambda: ops.distill_backward(x, stats, ids, teacher2, None, 1.0, up),
+           lambda: ops.distill_backward(x, stats, ids, teacher, None, 1.0, up2)][which]
+    with pytest.raises(ValueError, match="logit rows"):
+        bad()
+    assert launches == []
+
+
+@pytest.mark.parametrize("call", [
+    lambda x, tok, mask, ids, t: ops.token_logprobs_forward(x, tok.to(torch.int16), None, 0, 1.0, True, True),
+    lambda x, tok, mask, ids, t: ops.token_logprobs_forward(x, tok, mask.int(), 0, 1.0, True, True),
+    lambda x, tok, mask, ids, t: ops.distill_forward(x, ids.to(torch.int16), t, None, 1.0, True),
+    lambda x, tok, mask, ids, t: ops.distill_forward(x, ids, t, mask.long(), 1.0, True),
+])
+def test_functions_refuse_other_types(launches, call):
+    """Narrower ids would be read past their end, wider masks in pieces."""
+    with pytest.raises(TypeError, match="logit rows"):
+        call(*args()[:5])
+    assert launches == []
