@@ -167,6 +167,7 @@ class OutputHead(torch.nn.Module):
         if not self.fused():
             raise ValueError("token_loss: this head is not the fused RMSNorm + FP8 Einsum combination")
         lead = activations.shape[:-1]
+        self._check_width(activations, "token_loss")
         x2d = activations.to(torch.bfloat16).reshape(-1, self.model_d).contiguous()
         labels = targets.reshape(-1).to(torch.int32).contiguous()
         mk = None if mask is None else mask.reshape(-1).to(torch.uint8).contiguous()

@@ -417,11 +417,20 @@ def _pad16(n: int) -> int:
     return (n + 15) // 16 * 16
 
 
+def _check_labels(rows: int, labels: torch.Tensor, mask: torch.Tensor | None) -> None:
+    """The cross-entropy kernels read one int32 label and one mask byte per row."""
+    for name, t, size in (("labels", labels, 4), ("mask", mask, 1)):
+        if t is not None and (t.numel() != rows or t.element_size() != size):
+            raise ValueError(f"cross-entropy: {name} {tuple(t.shape)} {t.dtype} for {rows} rows (one value of {size} "
+                             f"bytes each)")
+
+
 def xent_rows(logits: torch.Tensor, labels: torch.Tensor, mask: torch.Tensor | None, V: int | None = None):
     """(lse, loss, qrow) f32 [rows] from bf16 logits [rows, >= V] (ufp8_xent_forward)."""
     if not logits.is_cuda or logits.dtype != torch.bfloat16 or (logits.numel() and logits.stride(1) != 1):
         raise ValueError("xent_rows: logits must be a CUDA bf16 tensor with unit column stride")
     rows = logits.shape[0]
+    _check_labels(rows, labels, mask)
     V = logits.shape[1] if V is None else V
     lse, loss, qrow = (torch.empty(rows, dtype=torch.float32, device=logits.device) for _ in range(3))
     ldl = logits.stride(0) if rows else V  # an empty tensor's strides carry no pitch
@@ -436,6 +445,7 @@ def xent_grad(logits: torch.Tensor, labels: torch.Tensor, mask: torch.Tensor | N
     """dlogits from bf16 logits (ufp8_xent_backward): a bf16 [rows, V] tensor for fmt BF16, else an
     Fp8Tensor [rows, Vp] (pitch Vp) with its per-tensor factors."""
     rows = logits.shape[0]
+    _check_labels(rows, labels, mask)
     V = logits.shape[1] if V is None else V
     dev = logits.device
     if fmt == C.BF16:
@@ -483,6 +493,7 @@ def xent_combine(stats: torch.Tensor, logits: torch.Tensor, V: int, labels: torc
                  mask: torch.Tensor | None):
     """(lse, loss, qrow) from the XENT epilogue's partials (ufp8_xent_combine)."""
     T, groups = stats.shape[0], stats.shape[1]
+    _check_labels(T, labels, mask)
     lse, loss, qrow = (torch.empty(T, dtype=torch.float32, device=logits.device) for _ in range(3))
     _launch("xent_combine", 8.0 * T * groups, lambda: C.xent_combine(
         stats.data_ptr(), groups, logits.data_ptr(), T, V, logits.stride(0), labels.data_ptr(),

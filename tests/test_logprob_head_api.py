@@ -48,6 +48,30 @@ def test_head_refuses_activations_of_another_width(head, shape):
             head.distillation_loss(x, fake(*lead, 4, dtype=torch.int64), fake(*lead, 4))
 
 
+def test_head_loss_refuses_activations_of_another_width():
+    """The loss of the same head flattens them in the same way."""
+    from macrogpt_jax_b200.einsum import Rngs
+    from macrogpt_jax_b200.head import OutputHead
+    h = OutputHead(D, V, rngs=Rngs(0))
+    with FakeTensorMode():
+        for width in (2 * D, D // 2):
+            with pytest.raises(ValueError, match="token_loss: activations"):
+                h.token_loss(fake(2, 3, width), fake(2, 3, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("n", [6, 13])
+def test_loss_functions_refuse_other_numbers_of_labels(n):
+    with FakeTensorMode():
+        x, row = fake(12, V), fake(12, dtype=torch.float32)
+        stats = fake(12, 1, 2, dtype=torch.float32)
+        good, lab, mk = fake(12, dtype=torch.int32), fake(n, dtype=torch.int32), fake(n, dtype=torch.uint8)
+        for labels, mask in ((lab, None), (good, mk), (fake(12, dtype=torch.int64), None)):
+            for call in (lambda: ops.xent_rows(x, labels, mask), lambda: ops.xent_combine(stats, x, V, labels, mask),
+                         lambda: ops.xent_grad(x, labels, mask, row, row, row, 0.0, C.E5M2)):
+                with pytest.raises(ValueError, match="cross-entropy"):
+                    call()
+
+
 ROWS = 12
 
 
