@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import ops
-from .logprobs import check_ids, check_logits, check_mask, check_temperature, first_order
+from .logprobs import check_ids, check_logits, check_mask, check_tangents, check_temperature, first_order
 
 MAX_ENTRIES = 1024
 
@@ -32,6 +32,7 @@ def check_teacher(teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, logit
         raise TypeError(f"{who}: expected bfloat16 or float32 teacher_logits, got {teacher_logits.dtype}")
     if torch.is_grad_enabled() and teacher_logits.requires_grad:
         raise ValueError(f"{who}: the teacher gets no gradient; detach teacher_logits")
+    check_tangents(who, teacher_logits)
     return ids, teacher_logits.detach().contiguous()
 
 
@@ -65,6 +66,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     keep gradients of one size across temperatures."""
     who = "topk_distillation_loss"
     check_logits(logits, who)
+    check_tangents(who, logits)
     temperature = check_temperature(temperature, who)
     ids, teacher = check_teacher(teacher_ids, teacher_logits, logits, who)
     mask = check_mask(mask, logits, who)

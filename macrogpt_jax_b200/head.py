@@ -28,8 +28,8 @@ from . import ops
 from .configurator import config
 from .einsum import Einsum, Rngs, zeros_init
 from .distill import check_teacher, topk_distillation_loss
-from .logprobs import (TokenLogprobs, check_ids, check_logits, check_mask, check_score, check_temperature, first_order,
-                       token_logprobs)
+from .logprobs import (TokenLogprobs, check_ids, check_logits, check_mask, check_score, check_tangents,
+                       check_temperature, first_order, token_logprobs)
 from .rmsnorm import RMSNorm
 
 HEAD_CAP = 15.0  # the constant of ueaj/model/model.py:163
@@ -182,12 +182,13 @@ class OutputHead(torch.nn.Module):
         if activations.shape[-1:] != (self.model_d,):
             raise ValueError(f"{who}: activations {tuple(activations.shape)}, expected [..., {self.model_d}]")
 
-    def _rows(self, activations: torch.Tensor, op):
+    def _rows(self, activations: torch.Tensor, op, who: str):
         """op's outputs on the logits of the flattened activations, through the fused node."""
         x2d = activations.to(torch.bfloat16).reshape(-1, self.model_d).contiguous()
         w = self.lm_head.w if self.lm_head.w.dtype == torch.bfloat16 else self.lm_head.w.to(torch.bfloat16)
         cap = HEAD_CAP if self.head_cap == "tanh" else 0.0
         scale = self.norm.scale
+        check_tangents(who, x2d, scale, w)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2d, scale, w)):
             return _HeadRowsFn.apply(x2d, scale, w, op, self.norm.recenter, self.norm.eps, cap,
                                      ops.FMT_OF_DTYPE[self.lm_head.bwd_dtype])
@@ -210,7 +211,7 @@ class OutputHead(torch.nn.Module):
             tokens = check_ids(tokens, lead, activations, "tokens", who).reshape(-1)
         mask = check_mask(mask, activations, who)
         op = _Score(tokens, None if mask is None else mask.reshape(-1), top_k, temperature, entropy)
-        lp, ent, top_lp, top_id = self._rows(activations, op)
+        lp, ent, top_lp, top_id = self._rows(activations, op, who)
         return TokenLogprobs(None if lp is None else lp.reshape(lead), None if ent is None else ent.reshape(lead),
                              None if top_lp is None else top_lp.reshape(*lead, top_k),
                              None if top_id is None else top_id.reshape(*lead, top_k))
@@ -231,4 +232,4 @@ class OutputHead(torch.nn.Module):
         K = ids.shape[-1]
         op = _Distill(ids.reshape(-1, K), teacher.reshape(-1, K), None if mask is None else mask.reshape(-1),
                       temperature)
-        return self._rows(activations, op)[0].reshape(lead)
+        return self._rows(activations, op, who)[0].reshape(lead)

@@ -14,6 +14,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -79,6 +80,15 @@ def check_ids(ids: torch.Tensor, shape, logits: torch.Tensor, name: str, who: st
     return ids.contiguous()
 
 
+def check_tangents(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses forward-mode derivatives, as an autograd function without one does; without the function
+    (nothing requires a gradient) the results would carry no tangent, that is, a derivative of zero."""
+    if forward_ad._current_level < 0:  # no dual tensors; unpack_dual says so too, in 0.9 us a tensor
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who}: forward-mode derivatives are not implemented")
+
+
 def first_order(backward):
     """once_differentiable, without its host time where no graph of the gradient is asked for."""
     once = torch.autograd.function.once_differentiable(backward)
@@ -127,6 +137,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     with other numbers of rows or another alignment, which group its sums differently."""
     who = "token_logprobs"
     check_logits(logits, who)
+    check_tangents(who, logits)
     lead, V = logits.shape[:-1], logits.shape[-1]
     temperature = check_score(tokens, top_k, V, temperature, entropy, who)
     if tokens is not None:

@@ -3,6 +3,7 @@ without a GPU: nothing may reach a kernel with fewer values than it has rows.  T
 CUDA device (shapes and types, no data) or CPU tensors that no check here lets through to a launch."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch._subclasses import FakeTensorMode
 
 from macrogpt_jax_b200 import _capi as C
@@ -70,6 +71,29 @@ def test_loss_functions_refuse_other_numbers_of_labels(n):
                          lambda: ops.xent_grad(x, labels, mask, row, row, row, 0.0, C.E5M2)):
                 with pytest.raises(ValueError, match="cross-entropy"):
                     call()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(grad):
+    """A tangent without requires_grad would be dropped: a derivative of zero without a word."""
+    from macrogpt_jax_b200.distill import topk_distillation_loss
+    from macrogpt_jax_b200.einsum import Rngs
+    from macrogpt_jax_b200.head import OutputHead
+    from macrogpt_jax_b200.logprobs import token_logprobs
+    h = OutputHead(D, V, rngs=Rngs(0)).requires_grad_(False)
+    with FakeTensorMode(allow_non_fake_inputs=True), forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        def dual(*shape, dtype=torch.float32):
+            return forward_ad.make_dual(fake(*shape, dtype=dtype), fake(*shape, dtype=dtype))
+        tok, ids, t = fake(2, dtype=torch.int64), fake(2, 3, dtype=torch.int64), fake(2, 3)
+        for call in (lambda: token_logprobs(dual(2, V), tok),
+                     lambda: topk_distillation_loss(dual(2, V), ids, t),
+                     lambda: topk_distillation_loss(fake(2, V), ids, dual(2, 3)),
+                     lambda: h.token_logprobs(dual(2, D, dtype=torch.bfloat16), tok),
+                     lambda: h.token_logprobs(dual(2, D), tok),
+                     lambda: h.distillation_loss(dual(2, D), ids, t),
+                     lambda: h.distillation_loss(fake(2, D), ids, dual(2, 3))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
 
 
 ROWS = 12
