@@ -177,6 +177,13 @@ class OutputHead(torch.nn.Module):
                                  ops.FMT_OF_DTYPE[self.lm_head.bwd_dtype])
         return loss.reshape(lead)
 
+    def _check_whole(self, who: str) -> None:
+        """With the lm_head's columns split over ranks (Einsum.reshard) the logits here are this rank's part."""
+        shard = getattr(self.lm_head, "shard", None)
+        if shard is not None:
+            raise NotImplementedError(f"{who}: the lm_head holds part {shard[1]} of {shard[2]} of the vocabulary; "
+                                      f"results over all of it are not implemented")
+
     def _check_width(self, activations: torch.Tensor, who: str) -> None:
         """Another width flattens to another number of rows than the tokens, ids and masks have."""
         if activations.shape[-1:] != (self.model_d,):
@@ -201,6 +208,7 @@ class OutputHead(torch.nn.Module):
         """logprobs.token_logprobs(self.get_logits(activations), ...), through the fused node when
         fused() holds (then the gradients reach the activations, the norm and the lm_head)."""
         who, lead = "OutputHead.token_logprobs", activations.shape[:-1]
+        self._check_whole(who)
         self._check_width(activations, who)
         if not self.fused():
             return token_logprobs(self.get_logits(activations), tokens, top_k=top_k, temperature=temperature, mask=mask,
@@ -221,6 +229,7 @@ class OutputHead(torch.nn.Module):
         """distill.topk_distillation_loss(self.get_logits(activations), ...), through the fused node when
         fused() holds."""
         who, lead = "OutputHead.distillation_loss", activations.shape[:-1]
+        self._check_whole(who)
         self._check_width(activations, who)
         if not self.fused():
             return topk_distillation_loss(self.get_logits(activations), teacher_ids, teacher_logits,

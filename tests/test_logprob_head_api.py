@@ -73,6 +73,32 @@ def test_loss_functions_refuse_other_numbers_of_labels(n):
                     call()
 
 
+def split_head(monkeypatch, rank=1, ranks=4):
+    """A head whose lm_head weight was split by Einsum.reshard, without a process group."""
+    import torch.distributed as dist
+    from macrogpt_jax_b200 import tp
+    from macrogpt_jax_b200.einsum import Rngs
+    from macrogpt_jax_b200.head import OutputHead
+    h = OutputHead(D, V, rngs=Rngs(0))
+    monkeypatch.setattr(tp, "tensor_group", lambda mesh: "group")
+    monkeypatch.setattr(dist, "get_world_size", lambda group: ranks)
+    monkeypatch.setattr(dist, "get_rank", lambda group: rank)
+    h.lm_head.reshard(object())
+    assert h.lm_head.w.shape == (D, V // ranks) and not h.fused()
+    return h
+
+
+def test_split_head_is_refused(monkeypatch):
+    """This rank's columns alone would give the entropy, alternatives and loss of a part of the vocabulary."""
+    h = split_head(monkeypatch)
+    with FakeTensorMode():
+        x, tok = fake(2, 3, D), fake(2, 3, dtype=torch.int64)
+        with pytest.raises(NotImplementedError, match="token_logprobs: the lm_head holds part 1 of 4"):
+            h.token_logprobs(x, tok)
+        with pytest.raises(NotImplementedError, match="distillation_loss: the lm_head holds part 1 of 4"):
+            h.distillation_loss(x, fake(2, 3, 4, dtype=torch.int64), fake(2, 3, 4))
+
+
 @pytest.mark.parametrize("grad", [True, False])
 def test_forward_mode_is_refused(grad):
     """A tangent without requires_grad would be dropped: a derivative of zero without a word."""
