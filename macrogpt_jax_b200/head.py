@@ -177,7 +177,7 @@ class OutputHead(torch.nn.Module):
                                  ops.FMT_OF_DTYPE[self.lm_head.bwd_dtype])
         return loss.reshape(lead)
 
-    def _check_whole(self, who: str) -> None:
+    def check_whole(self, who: str) -> None:
         """With the lm_head's columns split over ranks (Einsum.reshard) the logits here are this rank's part."""
         shard = getattr(self.lm_head, "shard", None)
         if shard is not None:
@@ -208,7 +208,7 @@ class OutputHead(torch.nn.Module):
         """logprobs.token_logprobs(self.get_logits(activations), ...), through the fused node when
         fused() holds (then the gradients reach the activations, the norm and the lm_head)."""
         who, lead = "OutputHead.token_logprobs", activations.shape[:-1]
-        self._check_whole(who)
+        self.check_whole(who)
         self._check_width(activations, who)
         if not self.fused():
             return token_logprobs(self.get_logits(activations), tokens, top_k=top_k, temperature=temperature, mask=mask,
@@ -229,7 +229,7 @@ class OutputHead(torch.nn.Module):
         """distill.topk_distillation_loss(self.get_logits(activations), ...), through the fused node when
         fused() holds."""
         who, lead = "OutputHead.distillation_loss", activations.shape[:-1]
-        self._check_whole(who)
+        self.check_whole(who)
         self._check_width(activations, who)
         if not self.fused():
             return topk_distillation_loss(self.get_logits(activations), teacher_ids, teacher_logits,

@@ -88,7 +88,10 @@ def softmax_cross_entropy_with_integer_labels(logits: torch.Tensor, labels: torc
 
 def _fused_head(logit_projection) -> Optional[OutputHead]:
     head = getattr(logit_projection, "__self__", logit_projection)
-    if not isinstance(head, OutputHead) or not head.fused():
+    if not isinstance(head, OutputHead):
+        return None
+    if not head.fused():
+        head.check_whole("chunked_softmax_cross_entropy")
         return None
     fn = getattr(logit_projection, "__func__", None)
     if logit_projection is head or fn in (OutputHead.get_logits, OutputHead.forward):

@@ -99,6 +99,17 @@ def test_split_head_is_refused(monkeypatch):
             h.distillation_loss(x, fake(2, 3, 4, dtype=torch.int64), fake(2, 3, 4))
 
 
+def test_loss_of_a_split_head_is_refused(monkeypatch):
+    """The same for the next-token loss, whichever way the head is given."""
+    from macrogpt_jax_b200.next_token_loss import chunked_softmax_cross_entropy
+    h = split_head(monkeypatch)
+    with FakeTensorMode():
+        x, tok = fake(2, 3, D), fake(2, 3, dtype=torch.int64)
+        for projection in (h, h.get_logits, h.forward):
+            with pytest.raises(NotImplementedError, match="cross_entropy: the lm_head holds part 1 of 4"):
+                chunked_softmax_cross_entropy(tok, x, projection)
+
+
 @pytest.mark.parametrize("grad", [True, False])
 def test_forward_mode_is_refused(grad):
     """A tangent without requires_grad would be dropped: a derivative of zero without a word."""
