@@ -238,7 +238,7 @@ class OutputHead(torch.nn.Module):
         temperature = check_temperature(temperature, who)
         ids, teacher = check_teacher(teacher_ids, teacher_logits, activations, who)
         mask = check_mask(mask, activations, who)
-        K = ids.shape[-1]
-        op = _Distill(ids.reshape(-1, K), teacher.reshape(-1, K), None if mask is None else mask.reshape(-1),
+        rows = (lead.numel(), ids.shape[-1])  # no -1, which fits any number of rows of no entries
+        op = _Distill(ids.reshape(rows), teacher.reshape(rows), None if mask is None else mask.reshape(-1),
                       temperature)
         return self._rows(activations, op, who)[0].reshape(lead)

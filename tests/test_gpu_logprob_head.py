@@ -233,3 +233,14 @@ def test_generic_head(cuda):
     loss = head.distillation_loss(x, out.top_ids, out.top_logprobs.detach())
     (loss.sum() - out.logprob.sum()).backward()
     assert x.grad.isfinite().all() and head.lm_head.w.grad.isfinite().all()
+
+
+def test_head_without_entries(cuda):
+    """No teacher entries: every loss is 0 and so are the gradients, as without the head."""
+    head, x, _ = make_head(cuda, 128, 512, "tanh", 9)
+    x = x.requires_grad_(True)
+    none = torch.empty((2, 48, 0), device=cuda)
+    loss = head.distillation_loss(x, none.long(), none)
+    assert loss.shape == (2, 48) and not loss.any()
+    loss.sum().backward()
+    assert not x.grad.any() and not head.lm_head.w.grad.any()

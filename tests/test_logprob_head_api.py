@@ -110,6 +110,22 @@ def test_loss_of_a_split_head_is_refused(monkeypatch):
                 chunked_softmax_cross_entropy(tok, x, projection)
 
 
+@pytest.mark.parametrize("lead", [(2, 3), (5,), (), (0,)])
+@pytest.mark.parametrize("k", [0, 1, 4])
+def test_head_takes_any_number_of_entries(monkeypatch, lead, k):
+    """No entries at all included, as topk_distillation_loss takes them."""
+    from macrogpt_jax_b200 import head as hd
+    from macrogpt_jax_b200.einsum import Rngs
+    seen = []
+    monkeypatch.setattr(hd.OutputHead, "_rows",
+                        lambda self, x, op, who: seen.append(op) or (x.new_empty(x.shape[:-1].numel()),))
+    h = hd.OutputHead(D, V, rngs=Rngs(0))
+    with FakeTensorMode():
+        loss = h.distillation_loss(fake(*lead, D), fake(*lead, k, dtype=torch.int64), fake(*lead, k))
+    rows = torch.Size(lead).numel()
+    assert loss.shape == lead and seen[0].ids.shape == (rows, k) and seen[0].teacher.shape == (rows, k)
+
+
 @pytest.mark.parametrize("grad", [True, False])
 def test_forward_mode_is_refused(grad):
     """A tangent without requires_grad would be dropped: a derivative of zero without a word."""
