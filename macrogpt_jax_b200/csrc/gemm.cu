@@ -1925,7 +1925,7 @@ int launch_gemm(const ufp8_gemm_desc& d, cudaStream_t stream, const DeviceInfo& 
   if (d.epilogue == UFP8_EPI_XENT) {
     if (d.d_dtype != UFP8_OUT_BF16 || d.batch != 1)
       return set_error(UFP8_ERR_INVALID, "XENT needs bf16 output and batch 1");
-    if (!d.xent_stats || d.xent_ld_stats < (d.N + 127) / 128)
+    if ((!d.xent_stats && d.M > 0) || d.xent_ld_stats < (d.N + 127) / 128)
       return set_error(UFP8_ERR_INVALID, "XENT needs xent_stats with xent_ld_stats >= ceil(N / 128)");
     if (reinterpret_cast<uintptr_t>(d.xent_stats) & 7u)
       return set_error(UFP8_ERR_ALIGN, "XENT: xent_stats is not 8-byte aligned");
@@ -1954,7 +1954,8 @@ int launch_gemm(const ufp8_gemm_desc& d, cudaStream_t stream, const DeviceInfo& 
   if ((d.epilogue == UFP8_EPI_SWIGLU || d.epilogue == UFP8_EPI_DSWIGLU) &&
       (d.d_dtype != UFP8_OUT_BF16 || d.batch != 1 || d.k_batches != 1))
     return set_error(UFP8_ERR_INVALID, "SWIGLU/DSWIGLU epilogues need bf16 output, batch 1, k_batches 1");
-  if (!d.d && !rs && d.epilogue != UFP8_EPI_ATTN_STATS) return set_error(UFP8_ERR_INVALID, "null output pointer");
+  const bool empty = d.M == 0 || d.N == 0;  // tensors without elements have no address
+  if (!empty && !d.d && !rs && d.epilogue != UFP8_EPI_ATTN_STATS) return set_error(UFP8_ERR_INVALID, "null output pointer");
   if (d.ldd < d.N) return set_error(UFP8_ERR_INVALID, "ldd < N");
   if (d.epilogue == UFP8_EPI_SWIGLU && (!d.h || d.ldh < d.N))
     return set_error(UFP8_ERR_INVALID, "SWIGLU needs h with ldh >= N");
@@ -1970,7 +1971,7 @@ int launch_gemm(const ufp8_gemm_desc& d, cudaStream_t stream, const DeviceInfo& 
     e = cudaMemsetAsync(d.amax_out, 0, sizeof(float), stream);
     if (e != cudaSuccess) return cuda_error(e, "cudaMemsetAsync(amax_out)");
   }
-  if (d.M == 0 || d.N == 0) return UFP8_OK;
+  if (empty) return UFP8_OK;
 
   GemmArgs a{};
   a.M = static_cast<int>(d.M);

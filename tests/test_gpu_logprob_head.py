@@ -244,3 +244,15 @@ def test_head_without_entries(cuda):
     assert loss.shape == (2, 48) and not loss.any()
     loss.sum().backward()
     assert not x.grad.any() and not head.lm_head.w.grad.any()
+
+
+def test_head_without_rows(cuda):
+    """No positions: empty results, and gradients of 0."""
+    head, x, _ = make_head(cuda, 128, 512, "tanh", 10)
+    x = x[:, :0].requires_grad_(True)
+    ids = torch.empty((2, 0, 4), dtype=torch.int64, device=cuda)
+    out = head.token_logprobs(x, ids[..., 0], top_k=3)
+    loss = head.distillation_loss(x, ids, torch.empty((2, 0, 4), device=cuda))
+    assert out.logprob.shape == out.entropy.shape == loss.shape == (2, 0) and out.top_ids.shape == (2, 0, 3)
+    (loss.sum() + out.logprob.sum()).backward()
+    assert x.grad.shape == x.shape and not head.lm_head.w.grad.any()
