@@ -69,10 +69,11 @@ class _HeadRowsFn(torch.autograd.Function):
         ids = [t for t in out if t is not None and not t.is_floating_point()]
         ctx.mark_non_differentiable(*ids)
         ctx.set_materialize_grads(False)
-        # all tensors through autograd, which frees them after the backward and notices a change in place
+        # all tensors through autograd, which frees them after the backward, notices a change in place and
+        # lets saved-tensor hooks move them; ctx.op keeps none
         ctx.save_for_backward(x2d, scale, logits, stats, rstd, qx.q, qx.inv_scale, qx.amax, qw.q, qw.inv_scale, qw.amax,
                               *ids, *op.tensors())
-        ctx.op, ctx.n_ids, ctx.V = op, len(ids), w.shape[1]
+        ctx.op, ctx.n_ids, ctx.V = op.with_tensors(*(None,) * len(op.tensors())), len(ids), w.shape[1]
         ctx.centered, ctx.cap, ctx.bwd_fmt = centered, cap, bwd_fmt
         return out
 
@@ -83,7 +84,8 @@ class _HeadRowsFn(torch.autograd.Function):
             return (None,) * 8
         x2d, scale, logits, stats, rstd, *rest = ctx.saved_tensors
         qx, qw, ids = ops.Fp8Tensor(*rest[:3]), ops.Fp8Tensor(*rest[3:6]), rest[6:6 + ctx.n_ids]
-        dxn, dw = ops.head_rows_backward(lambda lg, head: ctx.op.backward(lg, stats, ids, grads, head), logits,
+        op = ctx.op.with_tensors(*rest[6 + ctx.n_ids:])
+        dxn, dw = ops.head_rows_backward(lambda lg, head: op.backward(lg, stats, ids, grads, head), logits,
                                          (qx, rstd, qw), ctx.V, ctx.cap, ctx.needs_input_grad[2], ctx.bwd_fmt)
         need_ds = scale is not None and ctx.needs_input_grad[1]
         dx, ds = ops.rmsnorm_backward(x2d, scale, ctx.centered, rstd, dxn, need_ds)
@@ -101,6 +103,9 @@ class _Score(NamedTuple):
     def tensors(self):
         return self.tokens, self.mask
 
+    def with_tensors(self, tokens, mask):
+        return self._replace(tokens=tokens, mask=mask)
+
     def forward(self, logits, want_stats):
         *out, stats = ops.token_logprobs_forward(logits, self.tokens, self.mask, self.top_k, self.temperature,
                                                  self.entropy, want_stats)
@@ -109,7 +114,7 @@ class _Score(NamedTuple):
     def backward(self, logits, stats, ids, grads, head):
         dlp, dent, dtop, _ = grads
         return ops.token_logprobs_backward(logits, stats, self.tokens, self.mask, self.temperature, dlp, dent, dtop,
-                                    ids[0] if ids else None, head)
+                                           ids[0] if ids else None, head)
 
 
 class _Distill(NamedTuple):
@@ -120,6 +125,9 @@ class _Distill(NamedTuple):
 
     def tensors(self):
         return self.ids, self.teacher, self.mask
+
+    def with_tensors(self, ids, teacher, mask):
+        return self._replace(ids=ids, teacher=teacher, mask=mask)
 
     def forward(self, logits, want_stats):
         loss, stats = ops.distill_forward(logits, self.ids, self.teacher, self.mask, self.temperature, want_stats)

@@ -256,3 +256,34 @@ def test_head_without_rows(cuda):
     assert out.logprob.shape == out.entropy.shape == loss.shape == (2, 0) and out.top_ids.shape == (2, 0, 3)
     (loss.sum() + out.logprob.sum()).backward()
     assert x.grad.shape == x.shape and not head.lm_head.w.grad.any()
+
+
+def test_head_backward_reads_the_saved_tensors(cuda):
+    """The backward takes every input from autograd, so that saved-tensor hooks can move them: hooks that
+    hand back other tokens, teacher ids and masks than were saved give those tensors' gradient."""
+    head, x, g = make_head(cuda, 128, 512, "tanh", 11)
+    tok, tok2 = torch.randint(0, 512, (2, 2, 48), generator=g, device=cuda)
+    keep, keep2 = torch.rand((2, 2, 48), generator=g, device=cuda) > 0.3
+    ids, ids2 = torch.randint(0, 512, (2, 2, 48, 4), generator=g, device=cuda)
+    t, t2 = torch.randn((2, 2, 48, 4), generator=g, device=cuda)
+    x = x.requires_grad_(True)
+    swaps = {a.data_ptr(): b for a, b in ((tok, tok2), (keep, keep2), (ids, ids2), (t, t2))}
+
+    def unpack(s):
+        return swaps[s.data_ptr()].reshape(s.shape) if s.data_ptr() in swaps else s
+
+    def score(tok, keep):
+        return head.token_logprobs(x, tok, mask=keep, entropy=False).logprob
+
+    want, = torch.autograd.grad(score(tok2, keep & keep2).sum(), x)
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s, unpack):
+        # rows that were masked in the forward have no statistics
+        keep2 &= keep
+        got, = torch.autograd.grad(score(tok, keep).sum(), x)
+    assert torch.equal(got, want)
+    # the teacher's statistics are the forward's: other ids, the same values
+    swaps.pop(t.data_ptr())
+    want, = torch.autograd.grad(head.distillation_loss(x, ids2, t, mask=keep2).sum(), x)
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s, unpack):
+        got, = torch.autograd.grad(head.distillation_loss(x, ids, t, mask=keep).sum(), x)
+    assert torch.equal(got, want)
