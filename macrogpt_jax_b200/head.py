@@ -204,6 +204,11 @@ class OutputHead(torch.nn.Module):
         cap = HEAD_CAP if self.head_cap == "tanh" else 0.0
         scale = self.norm.scale
         check_tangents(who, x2d, scale, w)
+        if any(t is not None and t.device != x2d.device for t in (scale, w)):
+            raise ValueError(f"{who}: activations on {x2d.device}, the head on {w.device}")
+        if x2d.device.index != torch.cuda.current_device():  # the norm and the GEMMs launch on the current device
+            with torch.cuda.device(x2d.device):
+                return self._rows(activations, op, who)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2d, scale, w)):
             return _HeadRowsFn.apply(x2d, scale, w, op, self.norm.recenter, self.norm.eps, cap,
                                      ops.FMT_OF_DTYPE[self.lm_head.bwd_dtype])

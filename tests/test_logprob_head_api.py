@@ -126,6 +126,56 @@ def test_head_takes_any_number_of_entries(monkeypatch, lead, k):
     assert loss.shape == lead and seen[0].ids.shape == (rows, k) and seen[0].teacher.shape == (rows, k)
 
 
+def on(device, h):
+    """The head with fake parameters on the device."""
+    for m in (h.norm, h.lm_head):
+        for name, p in list(m.named_parameters()):
+            setattr(m, name, torch.nn.Parameter(torch.empty(p.shape, dtype=p.dtype, device=device)))
+    return h
+
+
+def test_head_runs_on_its_device(monkeypatch):
+    """Activations on another device than the current one: the whole node runs with that device current;
+    activations on another device than the head: refused."""
+    import contextlib
+    from macrogpt_jax_b200.einsum import Rngs
+    from macrogpt_jax_b200.head import OutputHead
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], torch.device(d).index
+        try:
+            yield
+        finally:
+            current[0] = before
+
+    def forward(x2d, scale, centered, eps, w, cap):
+        seen.append(current[0])
+        raise StopIteration
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(ops, "head_rows_forward", forward)
+    with FakeTensorMode():
+        h = OutputHead(D, V, rngs=Rngs(0))
+        x = torch.empty((2, D), dtype=torch.bfloat16, device="cuda:1")
+        tok = torch.empty(2, dtype=torch.int64, device="cuda:1")
+        ids, t = torch.empty((2, 3), dtype=torch.int64, device="cuda:1"), torch.empty((2, 3), device="cuda:1")
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                on("cuda:1", h)
+                for call in (lambda: h.token_logprobs(x, tok), lambda: h.distillation_loss(x, ids, t)):
+                    with pytest.raises(StopIteration):
+                        call()
+                    assert seen.pop() == 1 and current == [0]
+                on("cuda:0", h)
+                for call in (lambda: h.token_logprobs(x, tok), lambda: h.distillation_loss(x, ids, t)):
+                    with pytest.raises(ValueError, match="the head on cuda:0"):
+                        call()
+    assert not seen
+
+
 @pytest.mark.parametrize("grad", [True, False])
 def test_forward_mode_is_refused(grad):
     """A tangent without requires_grad would be dropped: a derivative of zero without a word."""
