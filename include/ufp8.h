@@ -41,7 +41,7 @@ extern "C" {
 
 typedef struct CUstream_st* ufp8_stream_t; /* same handle as cudaStream_t */
 
-#define UFP8_ABI_VERSION 6
+#define UFP8_ABI_VERSION 7
 
 /* return codes */
 #define UFP8_OK 0
@@ -66,6 +66,7 @@ typedef struct CUstream_st* ufp8_stream_t; /* same handle as cudaStream_t */
 #define UFP8_MN_MAJOR 1 /* stored [K][cols = M or N], M/N contiguous */
 
 #define UFP8_LIKE_LOGITS (-1) /* gradient of logit rows in the logits' own type */
+#define UFP8_AMAX_EXACT 16    /* added to its fp8 fmt: scale from the largest value itself, not from a bound */
 
 /* output element type */
 #define UFP8_OUT_BF16 0
@@ -323,7 +324,10 @@ int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens, int token
  * fmt UFP8_E4M3 / UFP8_E5M2 (bf16 logits, an output head's): *amax = the largest |dlogits| that the rows'
  * results allow (|dlogprob| + |dentropy| (1 / e + H) + sum |dtop|, over the temperature), s = FMAX / amax as
  * ufp8_quantize derives it, dlogits = fp8(dl * s), *inv_scale = 1 / s; cap > 0 says that the logits are
- * cap * tanh(l / cap) and asks for the gradient at l (times 1 - (x / cap)^2; UFP8_EPI_XENT's soft cap). */
+ * cap * tanh(l / cap) and asks for the gradient at l (times 1 - (x / cap)^2; UFP8_EPI_XENT's soft cap).
+ * The gradient can be thousands of times smaller than that bound.  e5m2 keeps its values' precision down to
+ * 2^-29.8 of it, e4m3 only to 2^-14.8: for e4m3 take UFP8_E4M3 + UFP8_AMAX_EXACT, where *amax is the largest
+ * |dlogits| itself (NaN if one of them is), found by one more pass over the logits. */
 int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const void* tokens, int token_bytes,
                           const float* dlogprob, int64_t dlogprob_stride, const float* dentropy,
                           int64_t dentropy_stride, const float* dtop, const int64_t* top_ids, int64_t top_k,
@@ -341,7 +345,8 @@ int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const vo
 int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teacher_ids, int id_bytes, const void* teacher,
                          int teacher_dtype, int64_t entries, float* loss, float* stats, ufp8_stream_t stream);
 /* dlogits[v] = dloss / temperature * (p_v - sum of q_j with id_j == v), 0 for rows with loss 0 by the
- * rules above; arguments as in ufp8_logprob_backward (fp8: *amax = max |dloss| / temperature).  The teacher
+ * rules above; arguments as in ufp8_logprob_backward (fp8: *amax = max |dloss| / temperature, or the
+ * largest |dlogits| with UFP8_AMAX_EXACT).  The teacher
  * gets no gradient. */
 int ufp8_distill_backward(const ufp8_logit_rows* x, const float* stats, const void* teacher_ids, int id_bytes,
                           const void* teacher, int teacher_dtype, int64_t entries, const float* dloss,

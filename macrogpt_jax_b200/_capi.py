@@ -17,6 +17,7 @@ IPC_HANDLE_BYTES = 64
 AG_COPY_ENGINE, AG_SM = 0, 1
 E4M3, E5M2 = 0, 1
 LIKE_LOGITS = -1  # output format of the logit-row gradients: the logits' own type
+AMAX_EXACT = 16  # added to its fp8 format: the scale from the largest value itself, not from a bound
 BF16 = 2  # bf16 GEMM operands; unquantised output of ufp8_xent_backward
 K_MAJOR, MN_MAJOR = 0, 1
 OUT_BF16, OUT_F32 = 0, 1

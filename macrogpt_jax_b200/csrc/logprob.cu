@@ -1005,9 +1005,10 @@ struct GradArgs {
   int K;
   const float* dloss;
   int64_t dloss_stride;
-  // fp8 output (an output head's logits): its format, 1 / cap of logits that are cap * tanh(.) (0: not
-  // capped), the bound of |output| and 1 / scale
+  // fp8 output (an output head's logits): its format, whether *amax is the largest |output| (else a bound of
+  // it), 1 / cap of logits that are cap * tanh(.) (0: not capped), and 1 / scale
   int fmt;
+  int exact;
   float inv_cap;
   float* amax;
   float* inv_scale;
@@ -1037,8 +1038,12 @@ __device__ __forceinline__ void load_entry(const GradArgs& a, int64_t row, int j
 }
 
 // The largest |dlogits| that the rows' results allow, and the fp8 scale from it: |p - [label]|, |p - q| and the
-// derivative of the soft cap are at most 1, and p |log p + H| <= 1 / e + H.  fp8's exponent covers the factor by
-// which that is too large.  One CTA; a NaN is above all.
+// derivative of the soft cap are at most 1, and p |log p + H| <= 1 / e + H.  The gradient itself can be thousands
+// of times smaller (an entropy bonus on flat rows, a student close to its teacher).  e5m2 covers that: an element
+// keeps its precision down to 2^-29.8 of the bound (2^-14 / 57344) and is lost below 2^-32.8, in sum at most 2^-15.8
+// of it in a row of 131072 columns.  e4m3 does not (2^-14.8 and 2^-18.8 of the bound; V 128256, normal logits,
+// entropy alone: 97 % of the elements flushed to 0); it goes with the measured amax (a.exact).  One CTA; a NaN is
+// above all.
 template <bool kDistill>
 __global__ void __launch_bounds__(1024) rowamax_kernel(const GradArgs a) {
   uint32_t top = 0;
@@ -1090,12 +1095,16 @@ __device__ __forceinline__ uint2 to_fp8(const float (&v)[8], int fmt) {
 // factors; per chunk it adds the weights of the row's entries that fall into it into `wt`, one f32 per
 // column and zero elsewhere, in entry order, so that the result does not depend on timing.  Then
 // v = p * factor + weight, and a lane with a weight in its columns sets those back to zero.
-// kHead: the logits are an output head's (bf16): the soft cap's derivative, and fp8 output by the scale of
-// rowamax_kernel.
-template <class T, bool kDistill, bool kHead>
+// kFp8: the logits are an output head's (bf16): the soft cap's derivative, and fp8 output by the scale of
+// rowamax_kernel, or, with a.exact, of the kAmax pass before this one: the same arithmetic on the same logits, which
+// keeps the largest |v| instead of storing.  The scale then multiplies the finished value, so that none of them
+// exceeds the format's largest; with the bound it goes into the factors.
+enum GradOut { kLike = 0, kFp8 = 1, kAmax = 2 };
+template <class T, bool kDistill, int kOut>
 __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) {
   constexpr int kChunk = 32 * kUnits;  // units of a chunk
   constexpr int kE = T::kElems;
+  constexpr bool kHead = kOut != kLike;
   extern __shared__ float4 wt_all[];    // kWarps * kChunk * kE floats
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float4* wt4 = wt_all + warp * kChunk * (kE / 4);
@@ -1106,7 +1115,12 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
   const int step_r = static_cast<int>(step / a.tasks), step_t = static_cast<int>(step % a.tasks);
   int row = static_cast<int>(first / a.tasks), task = static_cast<int>(first % a.tasks);
   const uint64_t c22 = pk(a.r.c2, a.r.c2), cap2 = pk(a.inv_cap, a.inv_cap);
-  const float sc = kHead ? scale_from_amax(*a.amax, a.fmt) : 1.0f;
+  const float scale = kOut == kFp8 ? scale_from_amax(*a.amax, a.fmt) : 1.0f;
+  const bool late = kOut == kFp8 && a.exact;
+  const float sc = late ? 1.0f : scale;
+  if (late && blockIdx.x == 0 && threadIdx.x == 0) *a.inv_scale = __fdiv_rn(1.0f, scale);
+  const uint64_t late2 = pk(scale, scale);
+  uint32_t top_bits = 0;  // kAmax: the largest |v| so far; a NaN is above all
   const int n = kDistill ? a.K : (a.dlogprob ? 1 : 0) + (a.dtop ? a.k : 0);
   if (n > 0)
     for (int i = lane; i < kChunk * (kE / 4); i += 32) wt4[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1121,7 +1135,7 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
     using Out = std::conditional_t<kHead, uint8_t, typename T::raw>;
     Out* o = static_cast<Out*>(a.out) + ri.elem(a.out_outer, a.out_inner);
     // the units' first elements lie on multiples of a unit in the output, too
-    const bool vec = ((reinterpret_cast<uintptr_t>(o) - x.off * sizeof(Out)) & (kE * sizeof(Out) - 1)) == 0;
+    const bool vec = kOut == kAmax || ((reinterpret_cast<uintptr_t>(o) - x.off * sizeof(Out)) & (kE * sizeof(Out) - 1)) == 0;
     const float4 st = a.stats[row];
     const bool dead = (a.r.mask && a.r.mask[row] == 0) || (kDistill && st.z == kNegInf);
     int u0 = task * a.per_task * kChunk;
@@ -1238,6 +1252,16 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
           }
         }
         const int c = x.col(i);
+        if constexpr (kOut == kAmax) {
+#pragma unroll
+          for (int j = 0; j < kE; ++j)
+            if (whole || (c + j >= 0 && c + j < x.V)) top_bits = max(top_bits, __float_as_uint(g[j]) & 0x7FFFFFFFu);
+          continue;
+        }
+        if (late) {
+#pragma unroll
+          for (int j = 0; j < kE; j += 2) unpk(mul2(pk(g[j], g[j + 1]), late2), g[j], g[j + 1]);
+        }
         // streaming stores: 4 % faster at 212 MB of gradient, 1 % at 1 GB
         if (whole || (vec && c >= 0 && c + kE <= x.V)) {
           if constexpr (kHead) {
@@ -1267,6 +1291,10 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
         }
       }
     }
+  }
+  if constexpr (kOut == kAmax) {
+    top_bits = __reduce_max_sync(0xFFFFFFFFu, top_bits);
+    if (lane == 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), top_bits);
   }
 }
 
@@ -1378,7 +1406,7 @@ int launch_stat(StatArgs& a, int dtype, const DeviceInfo& dev, cudaStream_t s) {
   return dtype == UFP8_OUT_F32 ? launch_stat<F32, kMode>(a, dev, s) : launch_stat<Bf16, kMode>(a, dev, s);
 }
 
-template <class T, bool kDistill, bool kHead>
+template <class T, bool kDistill, int kOut>
 int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
   constexpr int kChunk = 32 * kUnits;
   // a row that starts off a 16-byte boundary can need one unit more
@@ -1390,7 +1418,7 @@ int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
   if (dev_of[entries] != dev.device) {
     int n = 0;
     const cudaError_t e =
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rowgrad_kernel<T, kDistill, kHead>, kThreads, smem);
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rowgrad_kernel<T, kDistill, kOut>, kThreads, smem);
     if (e != cudaSuccess) return cuda_error(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor(row gradient)");
     per_sm[entries] = n < 1 ? 1 : n;
     dev_of[entries] = dev.device;
@@ -1401,26 +1429,34 @@ int launch_grad(GradArgs& a, const DeviceInfo& dev, cudaStream_t s) {
   while (a.per_task < 4 && a.per_task < chunks && a.r.rows * chunks >= cap * kWarps * 8 * a.per_task) a.per_task *= 2;
   a.tasks = static_cast<int>((chunks + a.per_task - 1) / a.per_task);
   const int64_t work = (a.r.rows * a.tasks + kWarps - 1) / kWarps;
-  rowgrad_kernel<T, kDistill, kHead><<<static_cast<unsigned>(work < cap ? work : cap), kThreads, smem, s>>>(a);
+  rowgrad_kernel<T, kDistill, kOut><<<static_cast<unsigned>(work < cap ? work : cap), kThreads, smem, s>>>(a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? UFP8_OK : cuda_error(e, "row gradient launch");
 }
 
 template <bool kDistill>
 int launch_grad(GradArgs& a, int dtype, const DeviceInfo& dev, cudaStream_t s) {
+  if (a.exact && a.r.rows > 0) {  // checked: fp8 output, bf16
+    const cudaError_t e = cudaMemsetAsync(a.amax, 0, sizeof(float), s);
+    if (e != cudaSuccess) return cuda_error(e, "cudaMemsetAsync(amax)");
+    if (int rc = launch_grad<Bf16, kDistill, kAmax>(a, dev, s)) return rc;
+    return launch_grad<Bf16, kDistill, kFp8>(a, dev, s);
+  }
   if (a.fmt != UFP8_LIKE_LOGITS) {  // checked: bf16
     rowamax_kernel<kDistill><<<1, 1024, 0, s>>>(a);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_error(e, "row amax launch");
-    return a.r.rows == 0 ? UFP8_OK : launch_grad<Bf16, kDistill, true>(a, dev, s);
+    return a.r.rows == 0 ? UFP8_OK : launch_grad<Bf16, kDistill, kFp8>(a, dev, s);
   }
-  return dtype == UFP8_OUT_F32 ? launch_grad<F32, kDistill, false>(a, dev, s)
-                               : launch_grad<Bf16, kDistill, false>(a, dev, s);
+  return dtype == UFP8_OUT_F32 ? launch_grad<F32, kDistill, kLike>(a, dev, s)
+                               : launch_grad<Bf16, kDistill, kLike>(a, dev, s);
 }
 
 // The output head's part of a backward: soft cap and fp8 output, for bf16 logits.
 int head_args(const ufp8_logit_rows* x, float cap, int fmt, float* amax, float* inv_scale, GradArgs* a,
               const char* who) {
+  const bool exact = fmt >= 0 && (fmt & UFP8_AMAX_EXACT);
+  if (exact) fmt &= ~UFP8_AMAX_EXACT;
   const bool fp8 = fmt == UFP8_E4M3 || fmt == UFP8_E5M2;
   if (!fp8 && fmt != UFP8_LIKE_LOGITS)
     return set_error(UFP8_ERR_INVALID, "%s: fmt %d is not UFP8_E4M3/UFP8_E5M2/UFP8_LIKE_LOGITS", who, fmt);
@@ -1432,6 +1468,7 @@ int head_args(const ufp8_logit_rows* x, float cap, int fmt, float* amax, float* 
   if (!al(amax, 4) || !al(inv_scale, 4))
     return set_error(UFP8_ERR_ALIGN, "%s: amax or inv_scale not 4-byte aligned", who);
   a->fmt = fmt;
+  a->exact = exact;
   a->inv_cap = cap > 0.0f ? 1.0f / cap : 0.0f;
   a->amax = amax;
   a->inv_scale = inv_scale;

@@ -15,8 +15,9 @@ recomputed, which the reference's rematerialised chunks do (one GEMM of 2 T d V 
 
 `token_logprobs` and `distillation_loss` put the operators of logprobs.py and distill.py behind the
 same head (the teacher's targets, the scores of sampled tokens, the student's step): one node of the
-same kind, whose backward writes the operator's logit gradient straight as fp8 (scale from the rows'
-results) and runs the two FP8 GEMMs and the norm's backward.
+same kind, whose backward writes the operator's logit gradient straight as fp8 (e5m2: scale from the
+rows' results; an e4m3 bwd_dtype: from the gradient's largest value, one more pass over the logits) and
+runs the two FP8 GEMMs and the norm's backward.
 """
 from __future__ import annotations
 

@@ -641,7 +641,7 @@ def _grad_target(lr: LogitRows, head: tuple | None):
         return (0.0, C.LIKE_LOGITS, *_grad_rows(lr), None, None)
     cap, fmt, pitch = head
     dev = lr.logits.device
-    out = torch.empty((lr.rows, pitch), dtype=FP8_DTYPE[fmt], device=dev)
+    out = torch.empty((lr.rows, pitch), dtype=FP8_DTYPE[fmt & ~C.AMAX_EXACT], device=dev)
     amax_t, inv = (torch.empty(1, dtype=torch.float32, device=dev) for _ in range(2))
     return cap, fmt, out, 0, pitch, amax_t, inv
 
@@ -683,7 +683,8 @@ def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: t
                             dent: torch.Tensor | None, dtop: torch.Tensor | None, top_id: torch.Tensor | None,
                             head: tuple | None = None) -> torch.Tensor | Fp8Tensor:
     """dlogits of token_logprobs_forward (ufp8_logprob_backward).  `head`: (soft cap, fp8 format, pitch) of
-    an output head: an Fp8Tensor [rows, pitch] of the gradient before the cap."""
+    an output head: an Fp8Tensor [rows, pitch] of the gradient before the cap, with the scale of a bound of it
+    or, with AMAX_EXACT in the format, of its largest value."""
     lr = logit_rows(logits)
     t = lr.logits
     dlp, s_lp = _row_grad(dlp, lr.rows)
@@ -733,8 +734,8 @@ def distill_backward(logits: torch.Tensor, stats: torch.Tensor, ids: torch.Tenso
 
 
 # The same operators behind the fused output head: final norm -> FP8 lm_head (soft cap in its epilogue) ->
-# logits [T, Vp] -> operator, whose gradient kernel writes fp8 dlogits for the two backward GEMMs (scale
-# from the rows' results, no pass over the gradient for its amax).
+# logits [T, Vp] -> operator, whose gradient kernel writes fp8 dlogits for the two backward GEMMs (e5m2: scale
+# from the rows' results, no pass for the amax; e4m3: one more pass over the logits for it).
 def head_rows_forward(x2d: torch.Tensor, scale: torch.Tensor | None, centered: bool, eps: float, w: torch.Tensor,
                       cap: float):
     """(logits bf16 [T, Vp] of which columns < V count, saved)."""
@@ -751,7 +752,8 @@ def head_rows_backward(grad_fn, logits: torch.Tensor, saved, V: int, cap: float,
     qx, _, qw = saved
     T, d = qx.q.shape
     Vp = logits.shape[1]
-    qd = grad_fn(logits[:, :V], (cap, fmt, Vp))
+    # e5m2 has the range for a scale from the rows' results alone; e4m3 loses the smaller values under it
+    qd = grad_fn(logits[:, :V], (cap, fmt if fmt == C.E5M2 else fmt | C.AMAX_EXACT, Vp))
     dxn = torch.empty((T, d), dtype=torch.bfloat16, device=logits.device)
     gemm(operand(qd, C.K_MAJOR, Vp), operand(qw, C.K_MAJOR, Vp), T, d, V, dxn, d)
     dw = None

@@ -252,3 +252,46 @@ def test_functions_refuse_other_types(launches, call):
     with pytest.raises(TypeError, match="logit rows"):
         call(*args()[:5])
     assert launches == []
+
+
+def test_exact_amax_flag():
+    """UFP8_AMAX_EXACT goes with the two fp8 formats, and with nothing else."""
+    import ctypes
+    import re
+    from pathlib import Path
+    header = (Path(__file__).resolve().parents[1] / "include" / "ufp8.h").read_text()
+    assert int(re.search(r"#define UFP8_AMAX_EXACT (\d+)", header)[1]) == C.AMAX_EXACT
+    p = 1 << 20  # stands for an aligned device address; no call here reads it
+    lib = C.load()
+
+    def call(fmt, dtype=C.OUT_BF16, cap=0.0, amax=p):
+        r = C.LogitRows(p, dtype, 1.0, 4, 100, 4, 0, 100, None)
+        a = lib.ufp8_logprob_backward(ctypes.byref(r), p, p, 8, p, 1, None, 0, None, None, 0, cap, fmt, p, 400, 100,
+                                      amax, p, None), lib.ufp8_last_error().decode()
+        b = lib.ufp8_distill_backward(ctypes.byref(r), p, p, 8, p, C.OUT_F32, 4, p, 1, cap, fmt, p, 400, 100, amax, p,
+                                      None), lib.ufp8_last_error().decode()
+        return a, b
+
+    for rc, msg in call(C.BF16 | C.AMAX_EXACT) + call(5 | C.AMAX_EXACT) + call(2 * C.AMAX_EXACT):
+        assert rc == C.ERR_INVALID and "fmt" in msg
+    for fmt in (C.E4M3, C.E5M2):
+        for rc, msg in call(fmt | C.AMAX_EXACT, dtype=C.OUT_F32):
+            assert rc == C.ERR_UNSUPPORTED and "bf16" in msg
+        for rc, msg in call(fmt | C.AMAX_EXACT, amax=None):
+            assert rc == C.ERR_INVALID and "null amax" in msg
+
+
+@pytest.mark.parametrize("fmt", [C.E4M3, C.E5M2])
+def test_head_backward_asks_for_the_scale_that_its_format_needs(monkeypatch, fmt):
+    """e5m2 takes the bound of the rows' results; e4m3, whose range it would use up, the largest value."""
+    asked = []
+
+    def grad(logits, head):
+        asked.append(head)
+        return ops.Fp8Tensor(torch.empty(3, 48, dtype=ops.FP8_DTYPE[fmt]), None, None)
+
+    monkeypatch.setattr(ops, "gemm", lambda *a, **k: None)
+    monkeypatch.setattr(ops, "operand", lambda *a: None)
+    q = ops.Fp8Tensor(torch.empty(3, D), None, None)
+    ops.head_rows_backward(grad, torch.empty(3, 48), (q, None, q), V, 15.0, True, fmt)
+    assert asked == [(15.0, C.E5M2 if fmt == C.E5M2 else C.E4M3 | C.AMAX_EXACT, 48)]
