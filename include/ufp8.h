@@ -309,9 +309,10 @@ typedef struct ufp8_logit_rows {
 /* Per row: logprob = log softmax[token], entropy = -sum p log p, and the top_k (0..256, <= V) largest
  * logits in descending order as (log probability, column), NaN first and ties to the lowest column.
  * tokens: int32 or int64 (token_bytes 4 / 8), a negative one counts from the end, one outside
- * [-V, V) gives NaN.  Any of the outputs may be NULL (tokens and logprob together).  A masked row
- * gives 0, 0, (-inf, -1).  A column of -inf has probability 0; a row of only -inf, or with +inf or
- * NaN, gives NaN.  One launch. */
+ * [-V, V) gives NaN (its gradient has no [v = token], as ufp8_xent_backward's for such a label:
+ * finite).  Any of the outputs may be NULL (tokens and logprob together).  A masked row gives 0, 0,
+ * (-inf, -1).  A column of -inf has probability 0; a row of only -inf, or with +inf or NaN, gives NaN.
+ * One launch. */
 int ufp8_logprob_forward(const ufp8_logit_rows* x, const void* tokens, int token_bytes, int64_t top_k,
                          float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids, float* stats,
                          ufp8_stream_t stream);
@@ -341,7 +342,8 @@ int ufp8_logprob_backward(const ufp8_logit_rows* x, const float* stats, const vo
  *   loss = sum_j q_j (log q_j - log p[id_j]),
  * the Kullback-Leibler divergence from the teacher's distribution renormalised over its entries.
  * Entries of -inf have q = 0; a row without any weight, or masked, has loss 0; an id >= V with q > 0
- * gives NaN.  A column given twice counts twice. */
+ * gives NaN (its q is left out of the gradient's sum, which stays finite).  A column given twice counts
+ * twice. */
 int ufp8_distill_forward(const ufp8_logit_rows* x, const void* teacher_ids, int id_bytes, const void* teacher,
                          int teacher_dtype, int64_t entries, float* loss, float* stats, ufp8_stream_t stream);
 /* dlogits[v] = dloss / temperature * (p_v - sum of q_j with id_j == v), 0 for rows with loss 0 by the

@@ -61,7 +61,8 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     `teacher_logits` [..., K] (bf16 or f32; log probabilities serve as well, since q does not change
     with a constant per row).  An entry of -inf has q = 0; a row without any weight has loss 0 and
     gradient 0, and so has a row whose `mask` [...] (bool or integer) is 0, which is not read.  An id >= V
-    with q > 0 gives NaN.  A column given twice counts twice.  The gradient reaches `logits` only, in
+    with q > 0 gives NaN, while the gradient, which has no column for it, stays finite with the other entries'
+    part: look at the loss.  A column given twice counts twice.  The gradient reaches `logits` only, in
     their type: (p_v - sum of q_j with id_j == v) / temperature; multiply the loss by temperature^2 to
     keep gradients of one size across temperatures."""
     who = "topk_distillation_loss"

@@ -126,7 +126,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     """Of every row of `logits` [..., V] (bf16 or f32, CUDA; any row strides, e.g. logits[:, :-1]), under
     the distribution p = softmax(logits / temperature):
       logprob       log p[token] for `tokens` [...] (integers; a negative token counts from the end, one
-                    outside [-V, V) gives NaN); None without tokens
+                    outside [-V, V) gives NaN, and its gradient is that of -log sum exp alone, as the
+                    next-token loss's is: finite, so look at the result); None without tokens
       entropy       -sum_v p_v log p_v (None with entropy=False)
       top_logprobs, top_ids   the top_k (at most 256) largest logits, descending: log p and column; NaN
                     first, ties to the lowest column

@@ -603,3 +603,33 @@ def test_long_rows_past_32_bits(cuda):
     ref, tol = grad_ref(x.detach()[-2:], tok[-2:], 1.0, torch.ones(2, device=cuda), None, None, None)
     check_grad(got[-2:], ref, tol)
     assert not got[:5].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_ids_without_a_column(cuda, dtype):
+    """A token outside [-V, V) and a teacher id >= V make their row's result NaN; the gradients leave them out
+    and stay finite, in that row and in all others."""
+    from macrogpt_jax_b200.distill import topk_distillation_loss
+    from macrogpt_jax_b200.logprobs import token_logprobs
+    V = 5001
+    x, tok, g = make(cuda, 8, V, dtype, 23)
+    tok[2], tok[5] = V, -V - 1
+    x = x.requires_grad_(True)
+    out = token_logprobs(x, tok, top_k=3)
+    assert torch.isnan(out.logprob).nonzero().flatten().tolist() == [2, 5]
+    assert out.entropy.isfinite().all() and out.top_logprobs.isfinite().all()
+    got, = torch.autograd.grad(out.logprob, x, torch.ones(8, device=cuda))
+    logp = torch.log_softmax(x.detach().double(), -1)
+    inside = (tok >= 0) & (tok < V)
+    ref = torch.zeros_like(logp).scatter_(1, tok.clamp(0, V - 1)[:, None], inside.double()[:, None]) - logp.exp()
+    check_grad(got, ref, logp.exp() * (lp_tol(logp, V) + 16 * U) + 4 * U * ref.abs())
+    ids = torch.rand((8, V), generator=g, device=cuda).argsort(-1)[:, :70]
+    t = torch.randn((8, 70), generator=g, device=cuda)
+    for row, j in ((1, 0), (4, 33), (6, 69)):
+        ids[row, j] = (V, V + 7, 2 ** 31 - 1)[row // 3]
+    for idt in (torch.int64, torch.int32):
+        loss = topk_distillation_loss(x, ids.to(idt), t, temperature=1.5)
+        assert torch.isnan(loss).nonzero().flatten().tolist() == [1, 4, 6]
+        got, = torch.autograd.grad(loss, x, torch.ones(8, device=cuda))
+        _, _, rg, gtol, _ = distill_ref(x.detach(), ids, t, 1.5)
+        check_grad(got, rg, gtol)
