@@ -1120,7 +1120,7 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
   const float sc = late ? 1.0f : scale;
   if (late && blockIdx.x == 0 && threadIdx.x == 0) *a.inv_scale = __fdiv_rn(1.0f, scale);
   const uint64_t late2 = pk(scale, scale);
-  uint32_t top_bits = 0;  // kAmax: the largest |v| so far; a NaN is above all
+  float largest = 0.0f;  // kAmax: |v| so far, NaN once one is
   const int n = kDistill ? a.K : (a.dlogprob ? 1 : 0) + (a.dtop ? a.k : 0);
   if (n > 0)
     for (int i = lane; i < kChunk * (kE / 4); i += 32) wt4[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1253,9 +1253,14 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
         }
         const int c = x.col(i);
         if constexpr (kOut == kAmax) {
+          if (whole) {
 #pragma unroll
-          for (int j = 0; j < kE; ++j)
-            if (whole || (c + j >= 0 && c + j < x.V)) top_bits = max(top_bits, __float_as_uint(g[j]) & 0x7FFFFFFFu);
+            for (int j = 0; j < kE; ++j) largest = maxn(largest, fabsf(g[j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < kE; ++j)
+              if (c + j >= 0 && c + j < x.V) largest = maxn(largest, fabsf(g[j]));
+          }
           continue;
         }
         if (late) {
@@ -1293,8 +1298,9 @@ __global__ void __launch_bounds__(kThreads, 4) rowgrad_kernel(const GradArgs a) 
     }
   }
   if constexpr (kOut == kAmax) {
-    top_bits = __reduce_max_sync(0xFFFFFFFFu, top_bits);
-    if (lane == 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), top_bits);
+    const uint32_t bits = __float_as_uint(largest) & 0x7FFFFFFFu;  // in the values' order, a NaN above all
+    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, bits);
+    if (lane == 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), top);
   }
 }
 
