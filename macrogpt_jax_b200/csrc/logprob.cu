@@ -13,11 +13,15 @@
 //   rowstat_kernel   one CTA per row (or a cluster of them) streams the row once, a running (m, s, t) per
 //                    thread, and notes where its largest elements may be; those are read again at the end.
 //                    Bound: HBM; next the ex2 of every logit (XU pipe 74 % busy).  4096 x 128256 bf16
-//                    (1.05 GB): 160 us for log probabilities, 164 with the entropy, 160 against 64 teacher
-//                    entries (6.4-6.6 TB/s), 216 with 64 alternatives; 1 x 128256: 3.7 us, 7.2 with 8.
+//                    (1.05 GB): 154-158 us for log probabilities, 162-164 with the entropy, 157-160 against 64
+//                    teacher entries (6.4-6.8 TB/s), 214-217 with 64 alternatives, 313 with 256; 1 x 128256:
+//                    3.7 us, 7.2 with 8.
 //   rowgrad_kernel   the gradient of both operators: p_v (A + B log2 p_v) with row factors A, B, plus
 //                    weights at a few columns (the token, the alternatives, the teacher's entries).
-//                    Bound: HBM, read and write.  Same size: 344 us (6.1 TB/s) for both.
+//                    Bound: HBM, read and write.  Same size: 336-347 us (6.1-6.3 TB/s) with up to 64 entries;
+//                    360 with 65, 387 with 128, 538 with 256, since each 2 KB of a row looks through all entries
+//                    past 64 again.  As fp8 (16384 x 128256, soft cap): 2.1 ms, 3.0 TB/s, bound by instructions;
+//                    the pass for the exact amax before it 1.2 ms.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -1042,8 +1046,9 @@ __device__ __forceinline__ void load_entry(const GradArgs& a, int64_t row, int j
 // of times smaller (an entropy bonus on flat rows, a student close to its teacher).  e5m2 covers that: an element
 // keeps its precision down to 2^-29.8 of the bound (2^-14 / 57344) and is lost below 2^-32.8, in sum at most 2^-15.8
 // of it in a row of 131072 columns.  e4m3 does not (2^-14.8 and 2^-18.8 of the bound; V 128256, normal logits,
-// entropy alone: 97 % of the elements flushed to 0); it goes with the measured amax (a.exact).  One CTA; a NaN is
-// above all.
+// entropy alone: 97 % of the elements flushed to 0); it goes with the measured amax (a.exact).  A NaN is above all.
+// One CTA, a thread per row: below 10 us at 16384 rows, but 2.3 ms with gradients of 256 alternatives each, whose
+// sums a thread reads alone.
 template <bool kDistill>
 __global__ void __launch_bounds__(1024) rowamax_kernel(const GradArgs a) {
   uint32_t top = 0;
@@ -1090,7 +1095,7 @@ __device__ __forceinline__ uint2 to_fp8(const float (&v)[8], int fmt) {
 }
 
 // The warps of a resident grid walk (row, task) units on their own, without a barrier (with one step per CTA all
-// waited for the warp that sorted the entries in: 458 us at 4096 x 128256 with 64 of them, 340 so); a task is
+// waited for the warp that sorted the entries in: 458 us at 4096 x 128256 with 64 of them, 336-347 so); a task is
 // `per_task` chunks of a row, a chunk 2 KB of it, kUnits 16-byte loads a lane.  Per task the warp works out the row
 // factors; per chunk it adds the weights of the row's entries that fall into it into `wt`, one f32 per
 // column and zero elsewhere, in entry order, so that the result does not depend on timing.  Then
@@ -1385,6 +1390,11 @@ int launch_stat(StatArgs& a, const DeviceInfo& dev, cudaStream_t s) {
   constexpr bool kTop = kMode == kTopK, kF32 = T::kKeyBits > 16;
   constexpr int kTile = 256 * kUnits * T::kElems;  // columns
   const int64_t rows = a.r.rows, V = a.r.V, sm = dev.sm_count, tiles = V / kTile;
+  // A sweep without alternatives (620-1900 rows x 2-20 tiles of columns, both types; 256 threads, two parts, 128
+  // threads) has the choice below within 5 % of the best of the three at 193 of 243 sizes, 1 % off on average.  The
+  // borders at 8 and 14 tiles lie between the sizes of the first sweep (3, 12, 15) and are not the best for f32 rows of
+  // 14 tiles and more, where one part of 256 (620 x 58709: 31.5 as chosen, 25.9) or 128 threads (1100 x 58709: 49.6,
+  // 43.8) would be faster, nor for 2 tiles of bf16 (1100 x 19114: 14.8, 12.8 with 128 threads).
   // Few rows: a row is split as long as its parts are whole tiles and all CTAs run at once (those that search for
   // alternatives take more of an SM).  1 x 128256: 11.7 / 3.7; 48: 12.2 / 5.7; 148: 12.4 / 10.9; 300: 21 / 19.
   int bits = 0;

@@ -54,7 +54,7 @@ class _DistillFn(torch.autograd.Function):
 
 def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
                            temperature: float = 1.0, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Per row of `logits` [..., V] (bf16 or f32, CUDA; any row strides) the f32 loss
+    """Per row of `logits` [..., V] (bf16 or f32, CUDA; strides as for token_logprobs) the f32 loss
       sum_j q_j (log q_j - log p[id_j]),   p = softmax(logits / temperature) over all V columns,
                                            q = softmax(teacher_logits / temperature) over the entries present,
     with `teacher_ids` [..., K] (integers, K <= 1024; an id < 0 marks an absent entry) and

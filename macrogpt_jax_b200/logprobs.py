@@ -123,8 +123,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
                    temperature: float = 1.0, mask: Optional[torch.Tensor] = None,
                    entropy: bool = True) -> TokenLogprobs:
-    """Of every row of `logits` [..., V] (bf16 or f32, CUDA; any row strides, e.g. logits[:, :-1]), under
-    the distribution p = softmax(logits / temperature):
+    """Of every row of `logits` [..., V] (bf16 or f32, CUDA; any strides), under the distribution
+    p = softmax(logits / temperature):
       logprob       log p[token] for `tokens` [...] (integers; a negative token counts from the end, one
                     outside [-V, V) gives NaN, and its gradient is that of -log sum exp alone, as the
                     next-token loss's is: finite, so look at the result); None without tokens
@@ -134,7 +134,10 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     `mask` [...] (bool or integer): a row whose mask is 0 is not read; it gives 0, 0, (-inf, -1) and a
     gradient of 0.  A logit of -inf has probability 0; a row of only -inf, or holding +inf or NaN, gives
     NaN.  Arithmetic is f32; gradients reach `logits` through logprob, entropy and top_logprobs, in the
-    logits' type.  The same call gives the same bits; the last bits of a row may differ between calls
+    logits' type.  Rows are read in place for up to two levels of row strides (logits[:, :-1], a padded
+    pitch); logits of more levels, or with a column stride, are copied, in the forward and in the backward.
+    For a next-token shift under autograd a mask of the last position is cheaper than logits[:, :-1], whose
+    own backward writes the whole gradient once more.  The same call gives the same bits; the last bits of a row may differ between calls
     with other numbers of rows or another alignment, which group its sums differently."""
     who = "token_logprobs"
     check_logits(logits, who)
