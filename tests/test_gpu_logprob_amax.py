@@ -160,3 +160,43 @@ def test_e4m3_head_gradients(cuda, cap, V, kind):
     dw = qx.reshape(-1, 256).T @ dl.reshape(-1, V)
     for a, b in ((x.grad, dx), (head.norm.scale.grad, ds), (head.lm_head.w.grad, dw)):
         compare(a.double().cpu().numpy(), b.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("fmt", [torch.float8_e4m3fn, torch.float8_e5m2])
+def test_head_step_replayed(cuda, fmt):
+    """The head's operators, forward and backward, captured and replayed on new inputs and run on another
+    stream: the same bits.  A larger gradient first, so that a stale largest value would show."""
+    from macrogpt_jax_b200.einsum import Einsum, Rngs
+    from macrogpt_jax_b200.graphs import GraphedStep
+    from macrogpt_jax_b200.head import OutputHead
+    head = OutputHead(128, 1000, lm_head=Einsum.override(bwd_dtype=fmt), rngs=Rngs(0))
+    g = torch.Generator(device=cuda).manual_seed(4)
+    with torch.no_grad():
+        head.lm_head.w.copy_(torch.randn((128, 1000), generator=g, device=cuda) / 11)
+    w = head.lm_head.w
+
+    def step(x, tok, ids, t, up):
+        x = x.detach().requires_grad_(True)
+        out = head.token_logprobs(x, tok, top_k=4)
+        loss = head.distillation_loss(x, ids, t)
+        return tuple(v.detach() for v in (*out, loss, *torch.autograd.grad((out.logprob, out.entropy), (x, w), (up, up)),
+                                          *torch.autograd.grad(loss, (x, w), up)))
+
+    def inputs(size):
+        return (torch.randn((2, 24, 128), generator=g, device=cuda).bfloat16(),
+                torch.randint(0, 1000, (2, 24), generator=g, device=cuda),
+                torch.randint(0, 1000, (2, 24, 6), generator=g, device=cuda),
+                torch.randn((2, 24, 6), generator=g, device=cuda),
+                size * torch.rand((2, 24), generator=g, device=cuda))
+
+    graphed = GraphedStep(step, *inputs(1.0))
+    for size in (100.0, 1e-3, 1.0):
+        args = inputs(size)
+        first = step(*args)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step(*args)
+        torch.cuda.current_stream().wait_stream(side)
+        for a, b, c in zip(first, other, graphed(*args)):
+            assert a.any() and torch.equal(a, b) and torch.equal(a, c)
