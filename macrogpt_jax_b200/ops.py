@@ -555,12 +555,13 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _dense(rows: int, *tensors: torch.Tensor | None, per_row: int = 1) -> None:
-    """The kernels index these by row: a tensor of another size would be read or written past its end."""
-    for t in tensors:
-        if t is not None and (t.numel() != rows * per_row or not t.is_contiguous()):
-            raise ValueError(f"logit rows: a tensor {tuple(t.shape)} with strides {t.stride()} where {rows} rows of "
-                             f"{per_row} values, contiguous, belong")
+def _dense(n: int, a: torch.Tensor | None, b: torch.Tensor | None = None) -> None:
+    """The kernels index these by row, n values in all: a tensor of another size would be read or written
+    past its end."""
+    if (a is None or (a.numel() == n and a.is_contiguous())) and (b is None or (b.numel() == n and b.is_contiguous())):
+        return
+    sizes = ", ".join(f"{tuple(t.shape)} with strides {t.stride()}" for t in (a, b) if t is not None)
+    raise ValueError(f"logit rows: {n} values, contiguous, belong to these rows, got {sizes}")
 
 
 def _id_bytes(t: torch.Tensor | None) -> int:
@@ -692,9 +693,9 @@ def token_logprobs_backward(logits: torch.Tensor, stats: torch.Tensor, tokens: t
     dtop = None if dtop is None else dtop.to(torch.float32).contiguous()
     top_k = top_id.shape[-1] if dtop is not None else 0
     _dense(lr.rows, tokens, mask)
-    _dense(lr.rows, stats, per_row=4)
+    _dense(4 * lr.rows, stats)
     if dtop is not None:
-        _dense(lr.rows, dtop, top_id, per_row=top_k)
+        _dense(top_k * lr.rows, dtop, top_id)
     cap, fmt, out, outer, inner, amax_t, inv = _grad_target(lr, head)
     _call_on(t, "logprob_grad", 2.0, C.logprob_backward, lr.c(temperature, mask), stats.data_ptr(), _ptr(tokens),
              _id_bytes(tokens), _ptr(dlp), s_lp, _ptr(dent), s_ent, _ptr(dtop), _ptr(top_id), top_k, cap,
@@ -706,13 +707,13 @@ def distill_forward(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tens
                     temperature: float, want_stats: bool):
     """(loss over the logits' leading shape, the backward's stats) (ufp8_distill_forward)."""
     lr = logit_rows(logits)
+    t, K = lr.logits, ids.shape[-1]
+    _dense(K * lr.rows, ids, teacher)
     _dense(lr.rows, mask)
-    _dense(lr.rows, ids, teacher, per_row=ids.shape[-1])
-    t = lr.logits
     loss = _empty_f32(logits.shape[:-1], t.device)
     stats = torch.empty(lr.rows, 4, dtype=torch.float32, device=t.device) if want_stats else None
     _call_on(t, "distill", 1.0, C.distill_forward, lr.c(temperature, mask), ids.data_ptr(), _id_bytes(ids),
-             teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], loss.data_ptr(), _ptr(stats))
+             teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype], K, loss.data_ptr(), _ptr(stats))
     return loss, stats
 
 
@@ -721,14 +722,14 @@ def distill_backward(logits: torch.Tensor, stats: torch.Tensor, ids: torch.Tenso
                      head: tuple | None = None) -> torch.Tensor | Fp8Tensor:
     """dlogits of distill_forward (ufp8_distill_backward); `head` as in token_logprobs_backward."""
     lr = logit_rows(logits)
+    t, K = lr.logits, ids.shape[-1]
+    _dense(K * lr.rows, ids, teacher)
+    _dense(4 * lr.rows, stats)
     _dense(lr.rows, mask)
-    _dense(lr.rows, ids, teacher, per_row=ids.shape[-1])
-    _dense(lr.rows, stats, per_row=4)
-    t = lr.logits
     dloss, stride = _row_grad(dloss, lr.rows)
     cap, fmt, out, outer, inner, amax_t, inv = _grad_target(lr, head)
     _call_on(t, "distill_grad", 2.0, C.distill_backward, lr.c(temperature, mask), stats.data_ptr(), ids.data_ptr(),
-             _id_bytes(ids), teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype], ids.shape[-1], dloss.data_ptr(), stride,
+             _id_bytes(ids), teacher.data_ptr(), _LOGIT_DTYPE[teacher.dtype], K, dloss.data_ptr(), stride,
              cap, fmt, out.data_ptr(), outer, inner, _ptr(amax_t), _ptr(inv))
     return out if head is None else Fp8Tensor(out, inv, amax_t)
 
